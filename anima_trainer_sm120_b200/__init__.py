@@ -5,6 +5,7 @@ modules here mirror the anima-trainer operator layer on top of it:
 
 * :mod:`.mxfp8_gemm`    quantiser + block-scaled GEMM (``mxfp8_gemm.py``)
 * :mod:`.adaln_kernel`  FusedAdaLN / FusedGatedAdd (``adaln_kernel.py``)
+* :mod:`.attention_kernel`  FusedAttention; :mod:`.qk_norm_rope` what comes before it
 * :mod:`.tlokr_kernels` rank_mix / rank_mix_wgrad (``tlokr_kernels.py``)
 * :mod:`.ops`           one thin wrapper per C entry point
 """

@@ -84,6 +84,15 @@ PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "anima_rmsnorm_rope_bwd_ex": (c_int, [P, P, P, c_int, P, P, P, I64, I64, I64, I64, P, P]),
     "anima_rmsnorm_rope_fwd": (c_int, [P, P, P, P, c_float, I64, I64, I64, I64, P, P, P]),
     "anima_rmsnorm_rope_bwd": (c_int, [P, P, P, P, P, P, I64, I64, I64, I64, P, P]),
+    "anima_qk_norm_rope_fwd": (c_int, [P, P, P, P, P, P, c_int, P, P, I64, c_float, *[I64] * 6, P, P, P]),
+    "anima_qk_norm_rope_bwd_workspace_bytes": (I64, [I64] * 6),
+    "anima_qk_norm_rope_bwd": (
+        c_int, [P, P, P, P, P, P, P, P, c_int, P, P, I64, c_float, *[I64] * 6, P, P, P, P, P, I64, P]),
+    "anima_attention_fwd_workspace_bytes": (I64, [*[I64] * 6, c_int]),
+    "anima_attention_fwd": (c_int, [P, P, P, P, P, P, P, *[I64] * 6, c_float, c_int, P, P, P, I64, P, P]),
+    "anima_attention_bwd_workspace_bytes": (I64, [*[I64] * 6, c_int]),
+    "anima_attention_bwd": (
+        c_int, [P, P, P, P, P, P, P, P, P, P, P, *[I64] * 6, c_float, c_int, P, P, P, P, I64, P, P]),
 }
 
 _lib: ctypes.CDLL | None = None
@@ -198,7 +207,7 @@ def check_status_word(device: torch.device) -> None:
     w = status_word(device)
     if int(w.item()) != 0:
         w.zero_()
-        raise RuntimeError("anima_mx_gemm: a bounded wait inside the kernel timed out")
+        raise RuntimeError("anima_mx_gemm / anima_attention: a bounded wait inside the kernel timed out")
 
 
 def check_quantize_status() -> None:

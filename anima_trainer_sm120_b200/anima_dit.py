@@ -15,6 +15,8 @@ Attribute and method names follow what the module patches read (``Block._forward
 
 Everything in this file is eager PyTorch (attention is torch SDPA, as in the reference): it is
 the "bf16 reference mode" arm and the host of the patched kernels, not itself a kernel.
+Padded texts: ``AnimaDiT.forward(..., context_lengths)`` hides the text tokens behind each sample's length
+from the cross-attention.
 """
 from __future__ import annotations
 
@@ -71,6 +73,13 @@ def apply_rotary_pos_emb(t: torch.Tensor, freqs: torch.Tensor) -> torch.Tensor:
     return t * cos + torch.cat((-t2, t1), dim=-1) * sin
 
 
+@dataclass(frozen=True)
+class AttentionParams:
+    """What a forward pass tells its attention layers: the number of text tokens of each sample (integers [B])."""
+
+    context_lengths: torch.Tensor
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: AnimaConfig, context_dim: int | None):
         super().__init__()
@@ -91,6 +100,18 @@ class Attention(nn.Module):
             q, k = apply_rotary_pos_emb(q, rope_emb), apply_rotary_pos_emb(k, rope_emb)
         return q, k
 
+    def _key_lengths(self, attn_params):
+        """Keys of each sample, or None where all count: lengths are those of the text, so of cross-attention only."""
+        return attn_params.context_lengths if self.is_cross and attn_params is not None else None
+
+    def _attend(self, q, k, v, attn_params=None):
+        """(B, L, H, d) queries, keys and values -> (B, L, H, d). ``attention_patch.install`` swaps in the fused kernels."""
+        lengths, mask = self._key_lengths(attn_params), None
+        if lengths is not None:
+            mask = (torch.arange(k.shape[1], device=k.device) < lengths[:, None])[:, None, None, :]
+        out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), attn_mask=mask)
+        return out.transpose(1, 2)
+
     def forward(self, x, attn_params=None, context=None, rope_emb=None):
         B, L, _ = x.shape
         ctx = x if context is None else context
@@ -98,8 +119,7 @@ class Attention(nn.Module):
         k = self.k_proj(ctx).view(B, ctx.shape[1], self.heads, self.head_dim)
         v = self.v_proj(ctx).view(B, ctx.shape[1], self.heads, self.head_dim)
         q, k = self._prepare_qk(q, k, None if self.is_cross else rope_emb)
-        out = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
-        return self.output_proj(out.transpose(1, 2).reshape(B, L, -1))
+        return self.output_proj(self._attend(q, k, v, attn_params).reshape(B, L, -1))
 
 
 class GPT2FeedForward(nn.Module):
@@ -237,8 +257,9 @@ class AnimaDiT(nn.Module):
         ang = F.pad(ang, (0, d // 2 - ang.shape[-1]))
         return torch.cat([ang, ang], dim=-1)[:, None, None, :]                       # (L, 1, 1, d)
 
-    def forward(self, x_B_C_T_H_W, timesteps_B, crossattn_emb, padding_mask=None):
+    def forward(self, x_B_C_T_H_W, timesteps_B, crossattn_emb, padding_mask=None, context_lengths=None):
         cfg = self.cfg
+        attn_params = None if context_lengths is None else AttentionParams(context_lengths)
         B, C, T, H, W = x_B_C_T_H_W.shape
         p = cfg.patch
         mask = torch.zeros(B, 1, T, H, W, device=x_B_C_T_H_W.device, dtype=x_B_C_T_H_W.dtype) \
@@ -249,7 +270,7 @@ class AnimaDiT(nn.Module):
         emb, adaln_lora = self.t_embedder(timesteps_B.view(B, 1).expand(B, T), x.dtype)
         rope = self._rope(T, H // p, W // p, x.device)
         for blk in self.blocks:
-            x = blk(x, emb, crossattn_emb, None, False, rope, adaln_lora, None)
+            x = blk(x, emb, crossattn_emb, attn_params, False, rope, adaln_lora, None)
         out = self.final_layer(x, emb)                                                # (B, T, h, w, p*p*C)
         out = out.view(B, T, H // p, W // p, cfg.latent_channels, p, p).permute(0, 4, 1, 2, 5, 3, 6)
         return out.reshape(B, cfg.latent_channels, T, H, W)

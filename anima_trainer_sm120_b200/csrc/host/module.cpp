@@ -3,6 +3,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include "attention.h"
 #include "linear.h"
 #include "norm.h"
 #include "tlokr.h"
@@ -129,4 +130,6 @@ PYBIND11_MODULE(_host, m) {
   ANIMA_DEF("gated_add", gated_add);
   ANIMA_DEF("gated_add_adaln", py_gated_add_adaln);
   ANIMA_DEF("rmsnorm_rope", rmsnorm_rope);
+  ANIMA_DEF("qk_norm_rope", qk_norm_rope);
+  ANIMA_DEF("attention", attention);
 }

@@ -72,6 +72,8 @@ def main() -> None:
     ap.add_argument("--variant", default="lokr", choices=["lokr", "tlokr"])
     ap.add_argument("--arms", default="bf16,mxfp8")
     ap.add_argument("--lr", type=float, default=1e-4)
+    ap.add_argument("--attention", default="sdpa", choices=["sdpa", "fused"],
+                    help="attention of the arms other than bf16: torch SDPA, or this package's kernels")
     ap.add_argument("--no-checkpoint", action="store_true",
                     help="keep every block's activations instead of recomputing them (the reference's configuration "
                          "recomputes; 180 GB of HBM leaves room not to)")
@@ -94,6 +96,7 @@ def main() -> None:
         torch.cuda.empty_cache()
         torch.cuda.reset_peak_memory_stats(dev)   # peak memory is reported per arm
         tr = Trainer(mcfg, StepConfig(precision=arm, variant=a.variant, lr=a.lr,
+                                       attention="sdpa" if arm == "bf16" else a.attention,
                                        gradient_checkpointing=not a.no_checkpoint), dev)
         losses, times = [], []
         for s in range(a.steps):

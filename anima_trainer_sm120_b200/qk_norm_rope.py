@@ -8,7 +8,8 @@ elementwise launches of the unpatched path. ``install`` patches ``Attention._pre
 way the reference's patches replace module methods; ``uninstall`` restores it.
 
 The fused path needs CUDA bf16 tensors with head width 128 and a frozen norm weight (adapter
-training); any other call keeps the original eager method.
+training); any other call keeps the original eager method. ``install(joint=True)`` runs the joint form instead
+(:func:`fused_qk_norm_rope`): q and k in ONE launch, head width 64 or 128, norm weights that may be trained.
 """
 from __future__ import annotations
 
@@ -41,6 +42,26 @@ class FusedRMSNormRoPE:
         return host().rmsnorm_rope(x, weight, cos, sin, eps)
 
 
+class FusedQKNormRoPE:
+    """``FusedRMSNormRoPE`` of the queries and the keys in one launch: heads of 64 or 128, as many key heads as there are, slices
+    of a packed projection read in place, gradients of the norm weights too (native: ``csrc/host/attention.cpp``)."""
+
+    @staticmethod
+    def apply(q, k, q_weight, k_weight, cos, sin, eps):
+        return host().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, eps)
+
+
+def fused_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                       cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, eps: float = 1e-6
+                       ) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(rope(rmsnorm(q) * q_weight), rope(rmsnorm(k) * k_weight))``, each head vector on its own.
+
+    ``q`` (B, Lq, H, D) and ``k`` (B, Lk, Hk, D) bfloat16, D 64 or 128, any strides; weights [D], bf16 or fp32; ``cos`` / ``sin``
+    fp32 [L, D], or [B, L, D] where the samples' tokens stand at positions of their own, or None (norm only). fp32 arithmetic,
+    rounded once; dense bfloat16 results. Gradients for q, k and the weights, not for the tables."""
+    return FusedQKNormRoPE.apply(q, k, q_weight, k_weight, cos, sin, eps)
+
+
 def _fusable(t: torch.Tensor, norm) -> bool:
     return (t.is_cuda and t.dtype == torch.bfloat16 and t.shape[-1] == 128 and t.dim() == 4
             and not norm.weight.requires_grad)
@@ -58,14 +79,22 @@ def _patched_prepare_qk(self, q, k, rope_emb):
             FusedRMSNormRoPE.apply(k, self.k_norm.weight, cos, sin, self.k_norm.eps))
 
 
-def install(attn_cls: type | None = None) -> None:
-    """Patch ``attn_cls._prepare_qk`` (default: the stand-in ``anima_dit.Attention``). Idempotent."""
+def _joint_prepare_qk(self, q, k, rope_emb):
+    if not (q.is_cuda and q.dtype == k.dtype == torch.bfloat16 and q.dim() == 4 and q.shape[-1] in (64, 128)
+            and self.q_norm.eps == self.k_norm.eps):
+        return _PATCHED[type(self)](self, q, k, rope_emb)
+    cos, sin = (None, None) if rope_emb is None else rope_tables(rope_emb)
+    return fused_qk_norm_rope(q, k, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.eps)
+
+
+def install(attn_cls: type | None = None, joint: bool = False) -> None:
+    """Patch ``attn_cls._prepare_qk`` (default: the stand-in ``anima_dit.Attention``): a launch each for q and k, or with
+    ``joint`` one for both. Idempotent; another call changes the form."""
     if attn_cls is None:
         from .anima_dit import Attention as attn_cls
-    if attn_cls in _PATCHED:
-        return
-    _PATCHED[attn_cls] = attn_cls._prepare_qk
-    attn_cls._prepare_qk = _patched_prepare_qk
+    if attn_cls not in _PATCHED:
+        _PATCHED[attn_cls] = attn_cls._prepare_qk
+    attn_cls._prepare_qk = _joint_prepare_qk if joint else _patched_prepare_qk
 
 
 def uninstall(attn_cls: type | None = None) -> None:

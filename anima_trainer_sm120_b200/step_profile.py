@@ -29,11 +29,12 @@ def main() -> None:
     ap.add_argument("--text", type=int, default=512)
     ap.add_argument("--top", type=int, default=30)
     ap.add_argument("--no-checkpoint", action="store_true")
+    ap.add_argument("--attention", default="sdpa", choices=["sdpa", "fused"])
     ap.add_argument("--gaps", type=int, default=0,
                     help="also list the N largest idle gaps between consecutive kernels (where the host fell behind)")
     a = ap.parse_args()
     dev = torch.device("cuda", 0)
-    tr = Trainer(AnimaConfig(depth=a.depth), StepConfig(precision=a.arm, variant=a.variant,
+    tr = Trainer(AnimaConfig(depth=a.depth), StepConfig(precision=a.arm, variant=a.variant, attention=a.attention,
                                                         gradient_checkpointing=not a.no_checkpoint), dev)
     for s in range(2):
         tr.step(*tr.synthetic_batch(a.batch, a.latent, a.text, s))

@@ -26,7 +26,7 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
-from . import adaln_kernel, adaln_merge, adaln_patch, lokr_patch, mlp_patch, precision, qk_norm_rope
+from . import adaln_kernel, adaln_merge, adaln_patch, attention_patch, lokr_patch, mlp_patch, precision, qk_norm_rope
 from .anima_dit import AnimaConfig, AnimaDiT, Attention, Block, GPT2FeedForward
 from .lokr import attach_lokr
 
@@ -56,6 +56,7 @@ class StepConfig:
     status_check_every: int = 1       # steps between reads of the kernels' bounded-wait status words (0 = never)
     cuda_graph: bool = False          # capture forward + backward per input shape and replay it (cuda_graphs.py)
     cuda_graph_warmup: int = 3
+    attention: str = "sdpa"           # "sdpa" (torch) | "fused": attention, q / k norm and rotation on this package's kernels
 
 
 class Trainer:
@@ -64,6 +65,10 @@ class Trainer:
     def __init__(self, model_cfg: AnimaConfig, cfg: StepConfig, device: torch.device):
         if cfg.precision not in ("bf16", "bf16_fused", "mxfp8"):
             raise ValueError(f"precision must be 'bf16', 'bf16_fused' or 'mxfp8', got {cfg.precision!r}")
+        if cfg.attention not in ("sdpa", "fused"):
+            raise ValueError(f"attention must be 'sdpa' or 'fused', got {cfg.attention!r}")
+        if cfg.attention == "fused" and cfg.precision == "bf16":
+            raise ValueError("attention='fused' needs precision 'bf16_fused' or 'mxfp8': 'bf16' is the eager arm")
         self.cfg, self.model_cfg, self.device = cfg, model_cfg, device
         self.world = dist.get_world_size() if dist.is_initialized() else 1
         self.rank = dist.get_rank() if dist.is_initialized() else 0
@@ -113,6 +118,11 @@ class Trainer:
             mlp_patch.uninstall(GPT2FeedForward)
             lokr_patch.disable_fp8()
             adaln_kernel.emit_row_operand(False)
+        if cfg.attention == "fused":
+            qk_norm_rope.install(Attention, joint=True)
+            attention_patch.install(Attention)
+        else:
+            attention_patch.uninstall(Attention)
         self.dit.train()
         self.params = [p for p in self.network.parameters() if p.requires_grad]
         # flat fp32 gradient buffer; every .grad is a view into it, so the DP exchange is one call
@@ -257,7 +267,7 @@ class Trainer:
             self.last_allreduce_exposed_ms = ev[0].elapsed_time(ev[1])
             self._exchange_events = None
         every = self.cfg.status_check_every
-        if self.cfg.precision == "mxfp8" and every and self.step_idx % every == 0:
+        if (self.cfg.precision == "mxfp8" or self.cfg.attention == "fused") and every and self.step_idx % every == 0:
             self.check_kernel_status()
         return value
 

@@ -439,6 +439,53 @@ int anima_rmsnorm_rope_bwd_ex(const void* dout, const void* x, const void* weigh
                               int64_t tokens, int64_t heads, int64_t head_dim, int64_t seq_len, void* dx,
                               void* stream);
 
+/* The queries and the keys in one launch, read where they lie, with the gradients of both norm weights.
+ * q [batch, lq, heads, head_dim], k [batch, lk, kv_heads, head_dim] bf16, head_dim 64 or 128; *_strides: HOST array of the
+ * three element strides (batch, token, head), multiples of 8; the head vector is dense. q_out, k_out dense. Weights
+ * [head_dim], both bf16 (weights_are_bf16 = 1) or both fp32. Tables fp32 [table_samples, lq, head_dim], table_samples 1 (shared by
+ * the samples) or batch, or both NULL; with tables lq == lk. fp32 math as above, rounded once.
+ * bwd: dq_out, dk_out dense bf16 gradients of the results; dq, dk dense bf16; dq_weight, dk_weight [head_dim] of the weights'
+ * type, either may be NULL (without both no workspace is needed). Fixed order of summation, no atomics. */
+int anima_qk_norm_rope_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                           const void* q_weight, const void* k_weight, int weights_are_bf16, const float* cos_tab,
+                           const float* sin_tab, int64_t table_samples, float eps, int64_t batch, int64_t lq, int64_t lk,
+                           int64_t heads, int64_t kv_heads, int64_t head_dim, void* q_out, void* k_out, void* stream);
+int64_t anima_qk_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
+                                               int64_t head_dim);
+int anima_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void* q, const int64_t* q_strides,
+                           const void* k, const int64_t* k_strides, const void* q_weight, const void* k_weight,
+                           int weights_are_bf16, const float* cos_tab, const float* sin_tab, int64_t table_samples,
+                           float eps, int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
+                           int64_t head_dim, void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- attention
+ * The DiT's attention between the prepared q / k and the output projection (the reference calls a library here).
+ *   s[i, j] = scale * q[i] . k[j];  p = softmax over the keys a query sees;  out[i] = sum_j p[i, j] v[j]
+ * q [batch, lq, heads, head_dim], k, v [batch, lk, kv_heads, head_dim] bf16, heads % kv_heads == 0 (a key head serves
+ * heads / kv_heads query heads in a row), head_dim 64 or 128; *_strides: HOST array of the three element strides (batch, token,
+ * head), multiples of 8. kv_lengths int32 [batch] or NULL: sample b has keys 0 .. kv_lengths[b] - 1 (clamped to 0 .. lk); what
+ * lies behind them is not used, whatever it holds. causal: query i sees keys j <= i + lk - lq. A query that sees no key has
+ * output 0 and lse -inf and no part in the gradients. scale > 0.
+ * out dense [batch, lq, heads, head_dim] bf16; lse fp32 [batch, heads, lq] (natural logarithm of the row's sum), NULL: not
+ * written (bwd needs it).
+ * bwd: dout as q; out and lse as fwd wrote them; dq like q, dk and dv like k, dense; any of them may be NULL. Deterministic.
+ * status: device int32 that a kernel raises if one of its bounded waits gave up, or NULL. */
+int64_t anima_attention_fwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
+                                            int64_t head_dim, int causal);
+int anima_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides, const int32_t* kv_lengths, int64_t batch, int64_t lq,
+                        int64_t lk, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
+                        void* out, float* lse, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+int64_t anima_attention_bwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
+                                            int64_t head_dim, int causal);
+int anima_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides,
+                        const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                        const void* out, const float* lse, const int32_t* kv_lengths, int64_t batch, int64_t lq,
+                        int64_t lk, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale, int causal,
+                        void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, int32_t* status,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif
