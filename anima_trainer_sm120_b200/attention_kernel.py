@@ -1,4 +1,4 @@
-"""Softmax attention as a fused autograd op on the sm_100a kernels of ``csrc/attention.cu``.
+"""Softmax attention as a fused autograd op on the sm_100a kernels of ``csrc/attention_fwd.cu`` and ``csrc/attention_bwd.cu``.
 
 anima-trainer leaves this step of the DiT to a library (``F.scaled_dot_product_attention``; its
 ``tests/bench_attention.py:3-7`` compares several). Tensors are (batch, tokens, heads, head_dim) as the projections

@@ -57,7 +57,7 @@ __device__ __forceinline__ int keys_of(const AttnParams& p, int b) {
 }
 
 // grid (ceil(lq / kWarps), heads, batch)
-template <int D, bool BWD>
+template <int D>
 __global__ void __launch_bounds__(kWarps * 32) attention_rows_kernel(const AttnParams p) {
   const int lane = threadIdx.x & 31, i = blockIdx.x * kWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
   if (i >= p.lq) return;
@@ -70,23 +70,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_rows_kernel(const AttnP
   load_vec<D>(p.q + b * p.sq.b + i * p.sq.l + h * p.sq.h, lane, q);
   const __nv_bfloat16* kp = p.k + b * p.sk.b + hk * p.sk.h;
   const __nv_bfloat16* vp = p.v + b * p.sv.b + hk * p.sv.h;
-  if (!BWD) {
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < n; ++j) {
-      load_vec<D>(kp + j * p.sk.l, lane, k);
-      load_vec<D>(vp + j * p.sv.l, lane, v);
-      const float s = dot<D>(q, k) * p.scale, mn = fmaxf(m, s), f = __expf(m - mn), e = __expf(s - mn);
-      l = l * f + e;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) acc[c] = acc[c] * f + e * v[c];
-      m = mn;
-    }
-    const float inv = n ? 1.f / l : 0.f;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) acc[c] *= inv;
-    store_vec<D>(p.o + dense, lane, acc);
-    if (p.lse && lane == 0) p.lse[row] = n ? m + logf(l) : -INFINITY;
-  } else {
+  {
     float g[D / 32], o[D / 32];
     load_vec<D>(p.dout + b * p.sdo.b + i * p.sdo.l + h * p.sdo.h, lane, g);
     load_vec<D>(p.out + dense, lane, o);
@@ -158,49 +142,6 @@ Strided strided(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
 using namespace anima;
 
-extern "C" int64_t anima_attention_fwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
-                                                       int64_t head_dim, int causal) {
-  (void)causal;
-  if (int rc = check_sizes("attention_fwd", batch, lq, lk, heads, kv_heads, head_dim)) return rc;
-  return 0;
-}
-
-extern "C" int anima_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                                   const void* v, const int64_t* v_strides, const int32_t* kv_lengths, int64_t batch,
-                                   int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
-                                   int causal, void* out, float* lse, void* workspace, int64_t workspace_bytes,
-                                   int32_t* status, void* stream) {
-  const char* who = "attention_fwd";
-  (void)workspace; (void)workspace_bytes; (void)status;
-  if (int rc = check_sizes(who, batch, lq, lk, heads, kv_heads, head_dim)) return rc;
-  ANIMA_REQUIRE(scale > 0.f && scale < INFINITY, ANIMA_E_ARG, "%s: scale must be positive and finite", who);
-  const bool no_q = batch * lq == 0, no_k = batch * lk == 0;
-  if (int rc = check_tensor(who, "q", q, q_strides, no_q)) return rc;
-  if (int rc = check_tensor(who, "k", k, k_strides, no_k)) return rc;
-  if (int rc = check_tensor(who, "v", v, v_strides, no_k)) return rc;
-  if (no_q) return ANIMA_OK;
-  ANIMA_REQUIRE(out, ANIMA_E_ARG, "%s: null pointer", who);
-  ANIMA_REQUIRE(aligned16(out), ANIMA_E_ALIGN, "%s: out must be 16-byte aligned", who);
-  AttnParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
-  p.v = static_cast<const __nv_bfloat16*>(v);
-  p.sq = strided(q_strides);
-  p.sk = strided(k_strides);
-  p.sv = strided(v_strides);
-  p.lengths = kv_lengths;
-  p.lq = (int)lq; p.lk = (int)lk; p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.causal = causal;
-  p.scale = scale;
-  p.lse = lse;
-  p.o = static_cast<__nv_bfloat16*>(out);
-  const dim3 grid((unsigned)ceil_div(lq, kWarps), (unsigned)heads, (unsigned)batch);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (head_dim == 64) attention_rows_kernel<64, false><<<grid, kWarps * 32, 0, s>>>(p);
-  else attention_rows_kernel<128, false><<<grid, kWarps * 32, 0, s>>>(p);
-  ANIMA_CHECK_LAUNCH(who);
-  return ANIMA_OK;
-}
-
 extern "C" int64_t anima_attention_bwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
                                                        int64_t head_dim, int causal) {
   (void)causal;
@@ -250,8 +191,8 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!no_q) {
     const dim3 grid((unsigned)ceil_div(lq, kWarps), (unsigned)heads, (unsigned)batch);
-    if (head_dim == 64) attention_rows_kernel<64, true><<<grid, kWarps * 32, 0, s>>>(p);
-    else attention_rows_kernel<128, true><<<grid, kWarps * 32, 0, s>>>(p);
+    if (head_dim == 64) attention_rows_kernel<64><<<grid, kWarps * 32, 0, s>>>(p);
+    else attention_rows_kernel<128><<<grid, kWarps * 32, 0, s>>>(p);
     ANIMA_CHECK_LAUNCH(who);
   }
   if (!no_k && (dk || dv)) {

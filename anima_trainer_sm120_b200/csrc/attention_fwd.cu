@@ -1,0 +1,460 @@
+// Attention, forward (formulas: attention_common.cuh): one pass over the keys with each row's running maximum and sum.
+//
+// A CTA owns two tiles of 128 queries of one head and walks the keys in tiles of 128. Per tile and key tile
+//   S = Q K^T     tcgen05, both operands in shared memory, fp32 scores in tensor memory (lane = query, column = key);
+//   softmax       one warpgroup a query tile, one thread a row: 128 scores into registers, row maximum without shuffles,
+//                 p = 2^(s scale log2 e - m), rounded to bf16 for the second product (the sum takes the unrounded values), written
+//                 over the scores;
+//   O += P V      tcgen05 with P read from tensor memory, V as it lies (keys along rows: the MN-major form), fp32.
+// The two tiles alternate: while one is in its softmax, the tensor cores work for the other. Warp 8 issues the products, warp
+// 9 feeds K and V tiles through a ring of TMA boxes.
+// The running maximum of a row is only raised once a score exceeds it by 2^8: until then p is at most 256, which costs neither
+// bf16 (relative) nor the fp32 sums anything, and O, which lies in tensor memory, need not be rescaled.
+// Few rows (one token, a short text) leave SMs idle: the keys are then cut into ranges, whose normalised fp32 outputs and
+// log-sums a second kernel joins in order. One query token per sample: the heads that share a key head become the rows of a
+// tile, so that each key is read once.
+// Bound: 4 D flop a (query, key) pair on the tensor cores and one exponential, of which an SM makes 16 a cycle: a tile
+// of D = 128 takes 1024 cycles of either.
+#include "attention_common.cuh"
+
+namespace anima {
+namespace attn {
+namespace {
+
+constexpr int kThreads = 320;            // two softmax warpgroups, one MMA warp, one TMA warp
+constexpr float kMaxSlack = 8.f;         // log2 of how far a score may exceed the maximum in use
+
+template <int D>
+struct FwdCfg {
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kBars = 2 * kStages + 7;
+  static constexpr int kSmem = (2 + kStages) * static_cast<int>(tile_bytes<D>()) + 1024 + kBars * 8 + 16;
+  // tensor-memory columns
+  static constexpr uint32_t kS = 0, kO = 256;
+};
+
+struct FwdParams {
+  Sizes z;
+  float c;                               // scale * log2 e
+  __nv_bfloat16* out;
+  Strided so;                            // of out
+  float* lse;                            // [batch, heads, lq] or null
+  int q_blocks, splits, tiles_per_split;
+  float* part_o;                         // [split][batch, heads, lq][D], null: no split
+  float* part_lse;                       // [split][batch, heads, lq], base 2
+  int64_t rows;                          // batch * heads * lq
+  int32_t* status;
+};
+
+// grid (q_blocks * splits, heads, batch)
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
+  using C = FwdCfg<D>;
+  constexpr uint32_t kBytes = tile_bytes<D>();
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ volatile int abort_flag;
+  __shared__ uint32_t tmem_slot;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  auto q_smem = [&](int t) { return base + t * kBytes; };
+  auto kv_smem = [&](int s) { return base + (2 + s) * kBytes; };
+  const uint32_t bars = base + (2 + C::kStages) * kBytes;
+  auto full = [&](int s) { return bars + 8 * s; };
+  auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
+  const uint32_t q_full = bars + 8 * (2 * C::kStages);
+  auto s_full = [&](int t) { return q_full + 8 * (1 + t); };
+  auto p_full = [&](int t) { return q_full + 8 * (3 + t); };
+  auto o_done = [&](int t) { return q_full + 8 * (5 + t); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(q_full, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(s_full(t), 1);
+      mbar_init(p_full(t), 4);
+      mbar_init(o_done(t), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+  }
+  if (warp == 8) tc_alloc(smem_u32(&tmem_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  after_previous();
+  const uint32_t tmem = tmem_slot;
+
+  const Sizes& z = p.z;
+  const int split = blockIdx.x / p.q_blocks, qb = blockIdx.x - split * p.q_blocks, h = blockIdx.y, b = blockIdx.z;
+  const int hk = h / z.group;
+  const int q0 = qb * 2 * kTile;
+  const int n = keys_of(z, b);
+  // key tiles this CTA walks for each query tile: [j0, j0 + count[t])
+  const int j0 = split * p.tiles_per_split;
+  int count[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int first = q0 + t * kTile;
+    const int last = min(z.lq, first + kTile) - 1;
+    const int lim = first < z.lq ? key_limit(z, n, last) : 0;
+    count[t] = max(0, min((lim + kTile - 1) / kTile, j0 + p.tiles_per_split) - j0);
+  }
+  const int most = max(count[0], count[1]);
+
+  if (warp == 9) {
+    // ------------------------------------------------------------ TMA producer: K0, V0, K1, V1, ...
+    if (lane == 0 && most > 0) {
+      mbar_expect_tx(q_full, kBytes * (count[1] > 0 ? 2 : 1));
+      load_tile<D>(q_smem(0), &map_q, q_full, q0, h, b);
+      if (count[1] > 0) load_tile<D>(q_smem(1), &map_q, q_full, q0 + kTile, h, b);
+      for (int i = 0; i < 2 * most; ++i) {
+        const int s = i % C::kStages;
+        if (!mbar_wait(empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
+        mbar_expect_tx(full(s), kBytes);
+        load_tile<D>(kv_smem(s), (i & 1) ? &map_v : &map_k, full(s), (j0 + (i >> 1)) * kTile, hk, b);
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr uint32_t kIdescS = tc_idesc_bf16(kTile, kTile), kIdescO = tc_idesc_bf16(kTile, D, true);
+    auto scores = [&](int t, int stage) {      // S_t = Q_t K^T
+      const uint64_t a = tc_desc_sw128(q_smem(t)), k = tc_desc_sw128(kv_smem(stage));
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t at = (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2;   // 16 bytes a unit
+        tc_mma_ss(tmem + C::kS + t * kTile, a + at, k + at, kIdescS, i > 0);
+      }
+      tc_commit(s_full(t));
+    };
+    bool ok = most > 0 && warp_wait(q_full, 0, &abort_flag) && warp_wait(full(0), 0, &abort_flag);
+    if (ok) {
+      tc_fence_after();
+      if (lane == 0) {
+        for (int t = 0; t < 2; ++t)
+          if (count[t] > 0) scores(t, 0);
+        tc_commit(empty(0));
+      }
+      __syncwarp();
+    }
+    for (int j = 0; j < most && ok; ++j) {
+      const int vi = 2 * j + 1, vs = vi % C::kStages, ki = 2 * j + 2, ks = ki % C::kStages;
+      // keys of the tile that exist; the product over the others is left out, up to the next multiple of 16
+      const int keys = min(kTile, n - (j0 + j) * kTile), steps = (keys + 15) / 16;
+      ok = warp_wait(full(vs), (vi / C::kStages) & 1, &abort_flag);
+      if (!ok) break;
+      if (keys & 15) zero_rows<D>(kv_smem(vs), keys, steps * 16);
+      const uint64_t v = tc_desc_sw128(kv_smem(vs), kTile * 128);
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (j >= count[t]) continue;
+        ok = warp_wait(p_full(t), j & 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t o = tmem + C::kO + t * D, pr = tmem + C::kS + t * kTile;
+          for (int i = 0; i < steps; ++i) tc_mma_ts(o, pr + i * 8, v + i * (16 * 128 / 16), kIdescO, j > 0 || i > 0);
+          tc_commit(o_done(t));
+        }
+        __syncwarp();
+        if (j + 1 < count[t]) {
+          ok = warp_wait(full(ks), (ki / C::kStages) & 1, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) scores(t, ks);
+          __syncwarp();
+        }
+      }
+      if (ok && lane == 0) {
+        tc_commit(empty(vs));
+        if (j + 1 < most) tc_commit(empty(ks));
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ softmax: warpgroup t, thread = row
+    const int t = warp >> 2;
+    const int row = q0 + t * kTile + (threadIdx.x & 127);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + C::kS + t * kTile, o_at = tmem + lanes + C::kO + t * D;
+    const int lim = key_limit(z, n, row);
+    // the warp's first row sees the fewest keys: tiles that end before that need no mask
+    const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
+    float m = -INFINITY, l = 0.f, used = 0.f;      // maximum in use (raw scores), sum, m * c (0 while there is none)
+    bool ok = true;
+    for (int j = 0; j < count[t]; ++j) {
+      ok = warp_wait(s_full(t), j & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tc_ld32(s_at + i * 32, s[i]);
+      tc_wait_ld();
+      const int k0 = (j0 + j) * kTile;
+      if (k0 + kTile > lim_all) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (k0 + i * 32 + e >= lim) s[i][e] = 0xff800000u;
+      }
+      float mx[4] = {m, m, m, m};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          mx[i] = fmaxf(mx[i], fmaxf(__uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1])));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool grow = (top - m) * p.c > kMaxSlack;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow ? exp2_approx((m - top) * p.c) : 1.f;      // 0 where there was no maximum yet
+        if (grow) {
+          m = top;
+          l *= f;
+          used = m * p.c;
+        }
+        if (j > 0) {
+          ok = warp_wait(o_done(t), (j - 1) & 1, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t o[32];
+            tc_ld32(o_at + i * 32, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tc_st32(o_at + i * 32, o);
+          }
+        }
+      }
+      const f2 c2 = f2_dup(p.c), u2 = f2_dup(-used);
+      f2 sum0 = 0ull, sum1 = 0ull;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const f2 x = f2_fma(f2_make(__uint_as_float(s[i][2 * e]), __uint_as_float(s[i][2 * e + 1])), c2, u2);
+          const f2 y = f2_make(exp2_approx(f2_lo(x)), exp2_approx(f2_hi(x)));
+          if (e & 1) sum1 = f2_add(sum1, y);
+          else sum0 = f2_add(sum0, y);
+          w[e] = bf16_of_f2(y);
+        }
+        tc_st16(s_at + i * 16, w);
+      }
+      l += f2_sum(f2_add(sum0, sum1));
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(t));
+    }
+    // ------------------------------------------------------------ epilogue
+    if (ok && count[t] > 0) {
+      ok = warp_wait(o_done(t), (count[t] - 1) & 1, &abort_flag);
+      tc_fence_after();
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;        // a row without keys has no sum
+    const bool live = row < z.lq && ok;
+    const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * z.lq + row;
+    const float total = l == 0.f ? -INFINITY : used + log2_approx(l);      // base 2
+    if (p.part_o != nullptr) {
+      if (live) p.part_lse[split * p.rows + at] = total;
+      if (count[t] > 0) {
+#pragma unroll 1
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t o[32];
+          __syncwarp();
+          tc_ld32(o_at + i * 32, o);
+          tc_wait_ld();
+          if (!live) continue;
+          float4* dst = reinterpret_cast<float4*>(p.part_o + (split * p.rows + at) * D + i * 32);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                                 __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+        }
+      }
+    } else {
+      if (live && p.lse) p.lse[at] = total * kLn2;
+      __nv_bfloat16* dst = p.out + b * p.so.b + row * p.so.l + h * p.so.h;
+#pragma unroll 1
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t o[32];
+        __syncwarp();
+        if (count[t] > 0) {
+          tc_ld32(o_at + i * 32, o);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float f[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[8 * e + x]) * inv;
+          *reinterpret_cast<uint4*>(dst + i * 32 + e * 8) = pack8(f);
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  if (abort_flag) {
+    // Copies still in flight land before shared memory is released.
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tc_dealloc(tmem, 512);
+  }
+}
+
+// out[row] = sum over splits of part_o[split][row] 2^(part_lse[split][row] - total), one warp a row, splits in ascending order.
+template <int D>
+__global__ void __launch_bounds__(256) attention_join_kernel(const __grid_constant__ FwdParams p) {
+  after_previous();
+  const int lane = threadIdx.x & 31;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (at >= p.rows) return;
+  const float* part_lse = after_previous(p.part_lse);
+  const float* part_o = after_previous(p.part_o);
+  float top = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, part_lse[s * p.rows + at]);
+  top = warp_max(top);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float acc[D / 32] = {}, l = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float w = part_lse[s * p.rows + at] - ref;
+    if (w == -INFINITY) continue;             // this range saw nothing and wrote nothing
+    const float f = exp2_approx(w);
+    l += f;
+    const float* src = part_o + (s * p.rows + at) * D + lane * (D / 32);
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) acc[e] = fmaf(f, src[e], acc[e]);
+  }
+  const int64_t bh = at / p.z.lq, row = at - bh * p.z.lq, b = bh / p.z.heads, h = bh - b * p.z.heads;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* dst = p.out + b * p.so.b + row * p.so.l + h * p.so.h + lane * (D / 32);
+#pragma unroll
+  for (int e = 0; e < D / 32; e += 2) *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
+  if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + log2_approx(l)) * kLn2;
+}
+
+// One query token a sample: the heads of a group become its tokens (nothing of the computation depends on a query's place: all
+// keys of the sample are seen).
+struct Shape {
+  int64_t batch, lq, lk, heads, kv_heads, d;
+  int causal;
+  bool regrouped = false;
+  Shape(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d, int causal)
+      : batch(batch), lq(lq), lk(lk), heads(heads), kv_heads(kv_heads), d(d), causal(causal) {
+    if (lq != 1) return;
+    this->causal = 0;
+    this->lq = heads / kv_heads;
+    this->heads = kv_heads;
+    regrouped = true;
+  }
+};
+
+// Ranges the keys are cut into: as many as give every SM two CTAs, none shorter than four tiles.
+int split_count(const Shape& s) {
+  const int64_t ctas = ceil_div(s.lq, 2 * kTile) * s.heads * s.batch, tiles = ceil_div(s.lk, kTile);
+  if (ctas == 0 || ctas >= sm_count()) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(2LL * sm_count(), ctas), tiles / 4)));
+}
+
+template <int D>
+int launch(const char* who, const CUtensorMap* maps, FwdParams p, const Shape& s, cudaStream_t st) {
+  using C = FwdCfg<D>;
+  static PerDeviceOnce once;
+  const cudaError_t rc = per_device_once(once, [] {
+    return cudaFuncSetAttribute(attention_fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  ANIMA_REQUIRE(rc == cudaSuccess, ANIMA_E_CUDA, "%s: cannot reserve %d bytes of shared memory: %s", who, C::kSmem,
+                cudaGetErrorString(rc));
+  const dim3 grid(static_cast<unsigned>(p.q_blocks * p.splits), static_cast<unsigned>(s.heads), static_cast<unsigned>(s.batch));
+  launch_after(attention_fwd_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], p);
+  ANIMA_CHECK_LAUNCH(who);
+  if (p.splits > 1) {
+    launch_after(attention_join_kernel<D>, dim3(static_cast<unsigned>(ceil_div(p.rows, 8))), dim3(256), 0, st, p);
+    ANIMA_CHECK_LAUNCH(who);
+  }
+  return ANIMA_OK;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace anima
+
+using namespace anima;
+
+extern "C" int64_t anima_attention_fwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
+                                                       int64_t head_dim, int causal) {
+  if (int rc = attn::check_sizes("attention_fwd", batch, lq, lk, heads, kv_heads, head_dim)) return rc;
+  const int64_t splits = attn::split_count(attn::Shape(batch, lq, lk, heads, kv_heads, head_dim, causal));
+  return splits > 1 ? splits * batch * heads * lq * (head_dim + 1) * 4 : 0;
+}
+
+extern "C" int anima_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                   const void* v, const int64_t* v_strides, const int32_t* kv_lengths, int64_t batch,
+                                   int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
+                                   int causal, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                   int32_t* status, void* stream) {
+  const char* who = "attention_fwd";
+  const int64_t need = anima_attention_fwd_workspace_bytes(batch, lq, lk, heads, kv_heads, head_dim, causal);
+  if (need < 0) return static_cast<int>(need);
+  ANIMA_REQUIRE(scale > 0.f && scale < INFINITY, ANIMA_E_ARG, "%s: scale must be positive and finite", who);
+  const bool no_q = batch * lq == 0, no_k = batch * lk == 0;
+  if (int rc = attn::check_tensor(who, "q", q, q_strides, no_q)) return rc;
+  if (int rc = attn::check_tensor(who, "k", k, k_strides, no_k)) return rc;
+  if (int rc = attn::check_tensor(who, "v", v, v_strides, no_k)) return rc;
+  if (no_q) return ANIMA_OK;
+  ANIMA_REQUIRE(out, ANIMA_E_ARG, "%s: null pointer", who);
+  ANIMA_REQUIRE(aligned16(out) && aligned16(workspace), ANIMA_E_ALIGN, "%s: out and workspace must be 16-byte aligned", who);
+  ANIMA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), ANIMA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed",
+                who, (long long)workspace_bytes, (long long)need);
+  const attn::Shape s(batch, lq, lk, heads, kv_heads, head_dim, causal);
+  attn::Strided sq = attn::strided(q_strides);
+  attn::FwdParams p = {};
+  p.so = {lq * heads * head_dim, heads * head_dim, head_dim};
+  if (s.regrouped) {
+    sq.l = sq.h;
+    sq.h = sq.l * s.lq;
+    p.so.l = head_dim;
+    p.so.h = head_dim * s.lq;
+  }
+  p.z = {static_cast<int>(s.lq), static_cast<int>(s.lk), static_cast<int>(s.heads), static_cast<int>(s.kv_heads),
+         static_cast<int>(s.heads / s.kv_heads), s.causal, kv_lengths};
+  p.c = scale * attn::kLog2e;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.status = status;
+  p.q_blocks = static_cast<int>(ceil_div(s.lq, 2 * attn::kTile));
+  p.splits = attn::split_count(s);
+  p.tiles_per_split = static_cast<int>(ceil_div(std::max<int64_t>(1, ceil_div(s.lk, attn::kTile)), p.splits));
+  p.rows = s.batch * s.heads * s.lq;
+  if (p.splits > 1) {
+    p.part_o = static_cast<float*>(workspace);
+    p.part_lse = p.part_o + p.splits * p.rows * head_dim;
+  }
+  CUtensorMap maps[3];
+  ANIMA_REQUIRE(attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, q) &&
+                    attn::encode_heads(&maps[1], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, q) &&
+                    attn::encode_heads(&maps[2], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, q),
+                ANIMA_E_CUDA, "%s: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand)", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return head_dim == 64 ? attn::launch<64>(who, maps, p, s, st) : attn::launch<128>(who, maps, p, s, st);
+}
