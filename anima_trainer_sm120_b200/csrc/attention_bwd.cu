@@ -1,152 +1,647 @@
-// Softmax attention over (batch, token, head, head_dim) tensors, forward and backward, bf16 in and out.
+// Attention, backward (formulas: attention_common.cuh): the probabilities are made again from q, k and the forward's log-sums.
 //
-//   s[i, j] = scale * q[i] . k[j],  p[i, j] = exp(s[i, j]) / sum over seen j' of exp(s[i, j']),  out[i] = sum_j p[i, j] v[j]
-//   lse[i]  = ln(sum_j exp(s[i, j]))
-//   delta[i] = out[i] . dout[i],    ds[i, j] = p[i, j] (dout[i] . v[j] - delta[i])
-//   dq[i] = scale * sum_j ds[i, j] k[j],  dk[j] = scale * sum_i ds[i, j] q[i],  dv[j] = sum_i p[i, j] dout[i]
-//
-// A key is seen by a query if it lies before the sample's length and, causal, at most lk - lq places after the query. A
-// query that sees no key has output 0 and lse -inf and takes no part in the gradients. kv_heads may divide heads.
-//
-// Plain form: one warp a query (or a key, for dk and dv), its head vector spread over the lanes, fp32 throughout.
-#include "common.cuh"
+// Three launches, no atomics, every sum in a fixed order:
+//   rows   delta = out . dout of each query, and its log-sum in base 2 (+inf for a query that saw nothing, and for the rows that
+//          fill up the last tile: their probabilities come out as 0);
+//   keys   one CTA a tile of 128 keys of a key head walks the query tiles of all heads it serves:
+//            S^T = K Q^T, dP^T = V dO^T (lane = key, column = query), dV += P^T dO, dK += dS^T Q;
+//   queries one CTA a tile of 128 queries of a head walks the key tiles:
+//            S = Q K^T, dP = dO V^T (lane = query), dQ += dS K.
+// That is 7 products a pair of tiles where one kernel for all three would do 5. It buys this: P^T, dS^T and dS are read by the
+// tensor cores from tensor memory, where the threads that made them wrote them over the scores, and never cross shared memory
+// (whose bandwidth a product with two operands there takes up whole); dQ needs no fp32 buffer that all CTAs add to (atomics
+// whose order would change results, and 4 bytes a key tile and element of traffic), and the sums stay in tensor memory.
+// Each tile of q, dO, K lies in shared memory once and serves as a K-major operand of one product and as an MN-major operand
+// of another.
+// Two warpgroups share a tile pair, 64 columns each; warp 8 issues the products so that the tensor cores work on the ones
+// that are ready while the warpgroups make the next probabilities: dV(i) and S(i+1) as soon as P(i) lies in tensor memory,
+// dK(i) and dP(i+1) as soon as dS(i) does.
+// Bound: 14 D flop a (query, key) pair on the tensor cores; two exponentials.
+#include "attention_common.cuh"
 
 namespace anima {
+namespace attn {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kThreads = 320;            // two warpgroups, one MMA warp, one TMA warp
 
-struct Strided {       // element strides of (batch, token, head); the head vector is dense
-  int64_t b, l, h;
-};
-struct AttnParams {
-  const __nv_bfloat16 *q, *k, *v, *out, *dout;
-  Strided sq, sk, sv, sdo;
-  const int32_t* lengths;
-  int lq, lk, heads, kv_heads, causal;
-  float scale;
-  float* lse;          // [batch, heads, lq]
-  float* delta;        // [batch, heads, lq]
-  __nv_bfloat16 *o, *dq, *dk, *dv;   // dense
+struct BwdParams {
+  Sizes z;
+  float c, scale;                        // scale * log2 e, scale
+  const float *lse2, *delta;             // [batch, heads, lq_pad]
+  int lq_pad;
+  __nv_bfloat16 *dq, *dk, *dv;
+  Strided sdq;                           // dk, dv: dense
+  int splits, per_split;                 // ranges of query tiles (keys) or key tiles (queries) a CTA takes
+  float *part0, *part1;                  // fp32 partial sums [split][elements], if splits > 1: dv and dk, or dq
+  int64_t elements;
+  int32_t* status;
 };
 
+struct RowsParams {
+  const __nv_bfloat16 *out, *dout;
+  Strided so, sdo;
+  const float* lse;
+  float *lse2, *delta;
+  int lq, lq_pad, heads;
+  int64_t rows;                          // batch * lq_pad * heads
+};
+
+// D / 8 lanes a row, rows in the order of memory
 template <int D>
-__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, int lane, float (&x)[D / 32]) {
-#pragma unroll
-  for (int e = 0; e < D / 32; e += 2) {
-    const float2 t = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p + lane * (D / 32) + e));
-    x[e] = t.x;
-    x[e + 1] = t.y;
-  }
-}
-template <int D>
-__device__ __forceinline__ void store_vec(__nv_bfloat16* p, int lane, const float (&x)[D / 32]) {
-#pragma unroll
-  for (int e = 0; e < D / 32; e += 2)
-    *reinterpret_cast<__nv_bfloat162*>(p + lane * (D / 32) + e) = __floats2bfloat162_rn(x[e], x[e + 1]);
-}
-template <int D>
-__device__ __forceinline__ float dot(const float (&a)[D / 32], const float (&b)[D / 32]) {
+__global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_constant__ RowsParams p) {
+  after_previous();
+  constexpr int kLanes = D / 8;
+  const int64_t r = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x & (kLanes - 1);
+  if (r >= p.rows) return;
+  const int h = static_cast<int>(r % p.heads);
+  const int64_t bl = r / p.heads, b = bl / p.lq_pad;
+  const int l = static_cast<int>(bl - b * p.lq_pad);
+  const int64_t to = (b * p.heads + h) * p.lq_pad + l;
   float s = 0.f;
+  if (l < p.lq) {
+    float x[8], y[8];
+    unpack8(*reinterpret_cast<const uint4*>(after_previous(p.out) + b * p.so.b + l * p.so.l + h * p.so.h + lane * 8), x);
+    unpack8(*reinterpret_cast<const uint4*>(after_previous(p.dout) + b * p.sdo.b + l * p.sdo.l + h * p.sdo.h + lane * 8), y);
 #pragma unroll
-  for (int e = 0; e < D / 32; ++e) s = fmaf(a[e], b[e], s);
-  return warp_sum(s);
-}
-__device__ __forceinline__ int keys_of(const AttnParams& p, int b) {
-  return p.lengths ? max(0, min(p.lk, p.lengths[b])) : p.lk;
+    for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(((1ull << kLanes) - 1) << (threadIdx.x & 31 & ~(kLanes - 1)), s, o);
+  if (lane != 0) return;
+  const float lse = l < p.lq ? after_previous(p.lse)[(b * p.heads + h) * p.lq + l] : -INFINITY;
+  p.lse2[to] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+  p.delta[to] = lse == -INFINITY ? 0.f : s;
 }
 
-// grid (ceil(lq / kWarps), heads, batch)
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) attention_rows_kernel(const AttnParams p) {
-  const int lane = threadIdx.x & 31, i = blockIdx.x * kWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
-  if (i >= p.lq) return;
-  const int hk = h / (p.heads / p.kv_heads);
-  int n = keys_of(p, b);
-  if (p.causal) n = max(0, min(n, i + p.lk - p.lq + 1));
-  const int64_t row = (static_cast<int64_t>(b) * p.heads + h) * p.lq + i;
-  const int64_t dense = ((static_cast<int64_t>(b) * p.lq + i) * p.heads + h) * D;
-  float q[D / 32], acc[D / 32] = {}, k[D / 32], v[D / 32];
-  load_vec<D>(p.q + b * p.sq.b + i * p.sq.l + h * p.sq.h, lane, q);
-  const __nv_bfloat16* kp = p.k + b * p.sk.b + hk * p.sk.h;
-  const __nv_bfloat16* vp = p.v + b * p.sv.b + hk * p.sv.h;
-  {
-    float g[D / 32], o[D / 32];
-    load_vec<D>(p.dout + b * p.sdo.b + i * p.sdo.l + h * p.sdo.h, lane, g);
-    load_vec<D>(p.out + dense, lane, o);
-    const float delta = dot<D>(g, o), lse = p.lse[row];
-    if (lane == 0) p.delta[row] = delta;
-    for (int j = 0; j < n; ++j) {
-      load_vec<D>(kp + j * p.sk.l, lane, k);
-      load_vec<D>(vp + j * p.sv.l, lane, v);
-      const float ds = __expf(dot<D>(q, k) * p.scale - lse) * (dot<D>(g, v) - delta) * p.scale;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(ds, k[c], acc[c]);
+struct BwdCfg {
+  static constexpr int kStages = D == 128 ? 4 : 8;                     // tiles in flight beside the two that stay
+  static constexpr int kBars = 2 * kStages + 8;
+  static constexpr int kRowBytes = 2 * kTile * 4;                      // lse2 and delta of a query tile
+  static constexpr int kSmem = (2 + kStages) * static_cast<int>(tile_bytes<D>()) + kStages / 2 * kRowBytes + 1024 + kBars * 8 + 16;
+  static constexpr uint32_t kS = 0, kDp = 128, kAcc0 = 256, kAcc1 = 256 + D;   // tensor-memory columns
+};
+
+// Shared memory and barriers of either kernel.
+template <int D>
+struct Layout {
+  using C = BwdCfg<D>;
+  uint32_t base;
+  __device__ __forceinline__ uint32_t fixed(int i) const { return base + i * tile_bytes<D>(); }
+  __device__ __forceinline__ uint32_t stage(int s) const { return base + (2 + s) * tile_bytes<D>(); }
+  __device__ __forceinline__ uint32_t row_data(int s) const { return base + (2 + C::kStages) * tile_bytes<D>() + (s >> 1) * C::kRowBytes; }
+  __device__ __forceinline__ uint32_t bars() const { return base + (2 + C::kStages) * tile_bytes<D>() + C::kStages / 2 * C::kRowBytes; }
+  __device__ __forceinline__ uint32_t full(int s) const { return bars() + 8 * s; }
+  __device__ __forceinline__ uint32_t empty(int s) const { return bars() + 8 * (C::kStages + s); }
+  __device__ __forceinline__ uint32_t bar(int i) const { return bars() + 8 * (2 * C::kStages + i); }
+};
+enum { kFixedFull, kSFull, kSFull1, kDpFull, kPReady, kDsReady, kDone };
+
+template <int D>
+__device__ __forceinline__ void setup(const Layout<D>& m, volatile int* abort_flag, uint32_t* tmem_slot, int warp) {
+  using C = BwdCfg<D>;
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(m.full(s), 1);
+      mbar_init(m.empty(s), 1);
     }
-    if (p.dq) store_vec<D>(p.dq + dense, lane, acc);
+    for (int i = kFixedFull; i <= kDone; ++i) mbar_init(m.bar(i), i == kPReady || i == kDsReady ? 8 : 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  after_previous();
+}
+__device__ __forceinline__ void teardown(volatile int* abort_flag, int32_t* status, uint32_t tmem, int warp) {
+  __syncwarp();
+  if (*abort_flag) {
+    // Copies still in flight land before shared memory is released.
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    if (threadIdx.x == 0 && status) atomicExch(status, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tc_dealloc(tmem, 512);
   }
 }
 
-// grid (ceil(lk / kWarps), kv_heads, batch)
+// D[tmem] (+)= A . B^T, both tiles in shared memory with the head vector along K
 template <int D>
-__global__ void __launch_bounds__(kWarps * 32) attention_keys_kernel(const AttnParams p) {
-  const int lane = threadIdx.x & 31, j = blockIdx.x * kWarps + (threadIdx.x >> 5), hk = blockIdx.y, b = blockIdx.z;
-  if (j >= p.lk) return;
-  float k[D / 32], v[D / 32], dk[D / 32] = {}, dv[D / 32] = {}, q[D / 32], g[D / 32];
-  const int group = p.heads / p.kv_heads;
-  if (j < keys_of(p, b)) {
-    load_vec<D>(p.k + b * p.sk.b + j * p.sk.l + hk * p.sk.h, lane, k);
-    load_vec<D>(p.v + b * p.sv.b + j * p.sv.l + hk * p.sv.h, lane, v);
-    for (int h = hk * group; h < (hk + 1) * group; ++h) {
-      const int64_t row = (static_cast<int64_t>(b) * p.heads + h) * p.lq;
-      for (int i = p.causal ? max(0, j - (p.lk - p.lq)) : 0; i < p.lq; ++i) {
-        load_vec<D>(p.q + b * p.sq.b + i * p.sq.l + h * p.sq.h, lane, q);
-        load_vec<D>(p.dout + b * p.sdo.b + i * p.sdo.l + h * p.sdo.h, lane, g);
-        const float e = __expf(dot<D>(q, k) * p.scale - p.lse[row + i]);
-        const float ds = e * (dot<D>(g, v) - p.delta[row + i]) * p.scale;
+__device__ __forceinline__ void product_ss(uint32_t d, uint32_t a_smem, uint32_t b_smem) {
+  const uint64_t a = tc_desc_sw128(a_smem), b = tc_desc_sw128(b_smem);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          dk[c] = fmaf(ds, q[c], dk[c]);
-          dv[c] = fmaf(e, g[c], dv[c]);
-        }
+  for (int i = 0; i < D / 16; ++i) {
+    const uint32_t at = (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2;     // 16 bytes a unit
+    tc_mma_ss(d, a + at, b + at, tc_idesc_bf16(kTile, kTile), i > 0);
+  }
+}
+// D[tmem] += A . B: A [128, 16 steps] bf16 in tensor memory, columns 0-63 at `a`, 64-127 at a + 64; B a tile with its rows along K
+template <int D>
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b_smem, int steps, bool accumulate) {
+  const uint64_t b = tc_desc_sw128(b_smem, kTile * 128);
+  for (int i = 0; i < steps; ++i)
+    tc_mma_ts(d, a + (i >> 2) * 64 + (i & 3) * 8, b + i * (16 * 128 / 16), tc_idesc_bf16(kTile, D, true), accumulate || i > 0);
+}
+
+// A thread's row of an fp32 accumulator, scaled: bf16 to dst, or fp32 to part (either may be null)
+template <int D>
+__device__ __forceinline__ void store_row(uint32_t acc, bool has, float scale, bool live, __nv_bfloat16* dst, float* part) {
+#pragma unroll 1
+  for (int i = 0; i < D / 32; ++i) {
+    uint32_t o[32];
+    __syncwarp();
+    if (has) {
+      tc_ld32(acc + i * 32, o);
+      tc_wait_ld();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0u;
+    }
+    if (!live) continue;
+    if (part) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        reinterpret_cast<float4*>(part + i * 32)[e] =
+            make_float4(__uint_as_float(o[4 * e]) * scale, __uint_as_float(o[4 * e + 1]) * scale,
+                        __uint_as_float(o[4 * e + 2]) * scale, __uint_as_float(o[4 * e + 3]) * scale);
+    } else if (dst) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[8 * e + x]) * scale;
+        *reinterpret_cast<uint4*>(dst + i * 32 + e * 8) = pack8(f);
       }
     }
   }
-  const int64_t dense = ((static_cast<int64_t>(b) * p.lk + j) * p.kv_heads + hk) * D;
-  if (p.dk) store_vec<D>(p.dk + dense, lane, dk);
-  if (p.dv) store_vec<D>(p.dv + dense, lane, dv);
 }
 
-int check_sizes(const char* who, int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-  ANIMA_REQUIRE(batch >= 0 && lq >= 0 && lk >= 0 && heads > 0 && kv_heads > 0, ANIMA_E_ARG, "%s: bad sizes", who);
-  ANIMA_REQUIRE(head_dim == 64 || head_dim == 128, ANIMA_E_UNSUPPORTED, "%s: head_dim=%lld is not supported (64 or 128)", who,
-                (long long)head_dim);
-  ANIMA_REQUIRE(heads % kv_heads == 0, ANIMA_E_SHAPE, "%s: heads=%lld is not a multiple of kv_heads=%lld", who,
-                (long long)heads, (long long)kv_heads);
-  ANIMA_REQUIRE(batch < 65536 && heads < 65536 && lq < (1ll << 30) && lk < (1ll << 30) && batch * heads * lq < (1ll << 40),
-                ANIMA_E_TOO_LARGE, "%s: too large", who);
+__device__ __forceinline__ float4 lds4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
+// ------------------------------------------------------------------------------------------------ keys: dK, dV
+// grid (key tiles * splits, kv_heads, batch)
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                          const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                          const __grid_constant__ BwdParams p) {
+  using C = BwdCfg<D>;
+  constexpr uint32_t kBytes = tile_bytes<D>();
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ volatile int abort_flag;
+  __shared__ uint32_t tmem_slot;
+  const Layout<D> m{(smem_u32(smem_raw) + 1023u) & ~1023u};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  setup<D>(m, &abort_flag, &tmem_slot, warp);
+  const uint32_t tmem = tmem_slot;
+
+  const Sizes& z = p.z;
+  const int split = blockIdx.x % p.splits, jt = blockIdx.x / p.splits, hk = blockIdx.y, b = blockIdx.z;
+  const int k0 = jt * kTile, n = keys_of(z, b), off = z.lk - z.lq;
+  const int q_tiles = (z.lq + kTile - 1) / kTile;
+  const int first = z.causal ? min(q_tiles, max(0, k0 - off) / kTile) : 0;     // the first query tile with a row that sees a key here
+  const int per_head = k0 < n ? q_tiles - first : 0;
+  const int begin = split * p.per_split, count = max(0, min(z.group * per_head, begin + p.per_split) - begin);
+  // pass i of this CTA: query tile `tile(i)` of head `head(i)`
+  auto head = [&](int i) { return hk * z.group + (begin + i) / per_head; };
+  auto tile = [&](int i) { return first + (begin + i) % per_head; };
+
+  if (warp == 9) {
+    // ------------------------------------------------------------ TMA producer: Q0 (with lse2, delta), dO0, Q1, ...
+    if (lane == 0 && count > 0) {
+      mbar_expect_tx(m.bar(kFixedFull), 2 * kBytes);
+      load_tile<D>(m.fixed(0), &map_k, m.bar(kFixedFull), k0, hk, b);
+      load_tile<D>(m.fixed(1), &map_v, m.bar(kFixedFull), k0, hk, b);
+      for (int i = 0; i < 2 * count; ++i) {
+        const int s = i % C::kStages, h = head(i >> 1), q0 = tile(i >> 1) * kTile;
+        if (!mbar_wait(m.empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
+        if (i & 1) {
+          mbar_expect_tx(m.full(s), kBytes);
+          load_tile<D>(m.stage(s), &map_do, m.full(s), q0, h, b);
+        } else {
+          mbar_expect_tx(m.full(s), kBytes + C::kRowBytes);
+          load_tile<D>(m.stage(s), &map_q, m.full(s), q0, h, b);
+          const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + q0;
+          bulk_load(m.row_data(s), p.lse2 + at, kTile * 4, m.full(s));
+          bulk_load(m.row_data(s) + kTile * 4, p.delta + at, kTile * 4, m.full(s));
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA issuer
+    // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
+    // share with others their rows are cleared, so that whatever q and dout hold there meets a probability of 0 as 0.
+    auto wait_stage = [&](int i) {
+      if (!warp_wait(m.full(i % C::kStages), (i / C::kStages) & 1, &abort_flag)) return false;
+      if (z.causal && tile(i >> 1) * kTile < -off) zero_rows<D>(m.stage(i % C::kStages), 0, -off - tile(i >> 1) * kTile);
+      return true;
+    };
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && wait_stage(0);
+    if (ok) {
+      tc_fence_after();
+      if (lane == 0) {
+        product_ss<D>(tmem + C::kS, m.fixed(0), m.stage(0));
+        tc_commit(m.bar(kSFull));
+      }
+      ok = wait_stage(1);
+      tc_fence_after();
+      if (ok && lane == 0) {
+        product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage(1));
+        tc_commit(m.bar(kDpFull));
+      }
+      __syncwarp();
+    }
+    for (int i = 0; i < count && ok; ++i) {
+      const int qs = 2 * i % C::kStages, gs = (2 * i + 1) % C::kStages;
+      const bool more = i + 1 < count;
+      ok = warp_wait(m.bar(kPReady), i & 1, &abort_flag) && (!more || wait_stage(2 * i + 2));
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        product_ts<D>(tmem + C::kAcc0, tmem + C::kS, m.stage(gs), kTile / 16, i > 0);
+        tc_commit(m.empty(gs));
+        if (more) {
+          product_ss<D>(tmem + C::kS, m.fixed(0), m.stage((2 * i + 2) % C::kStages));
+          tc_commit(m.bar(kSFull));
+        }
+      }
+      __syncwarp();
+      ok = warp_wait(m.bar(kDsReady), i & 1, &abort_flag) && (!more || wait_stage(2 * i + 3));
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        product_ts<D>(tmem + C::kAcc1, tmem + C::kDp, m.stage(qs), kTile / 16, i > 0);
+        if (more) {
+          tc_commit(m.empty(qs));
+          product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage((2 * i + 3) % C::kStages));
+          tc_commit(m.bar(kDpFull));
+        } else {
+          tc_commit(m.bar(kDone));
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ probabilities: thread = key, warpgroup w has 64 queries
+    const int w = warp >> 2, row = k0 + (threadIdx.x & 127);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + C::kS + w * 64, dp_at = tmem + lanes + C::kDp + w * 64;
+    const bool row_ok = row < n;
+    bool ok = true;
+    const f2 c2 = f2_dup(p.c), minus = f2_dup(-1.f);
+    for (int i = 0; i < count; ++i) {
+      const int qs = 2 * i % C::kStages;
+      const int q0 = tile(i) * kTile + w * 64;
+      const uint32_t rows = m.row_data(qs) + w * 256;
+      ok = warp_wait(m.full(qs), (2 * i / C::kStages) & 1, &abort_flag) && warp_wait(m.bar(kSFull), i & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[2][32];
+      tc_ld32(s_at, s[0]);
+      tc_ld32(s_at + 32, s[1]);
+      tc_wait_ld();
+      // queries of this tile before `from` do not see this key
+      const int from = !row_ok ? 64 : (z.causal ? row - off - q0 : 0);
+      const bool edge = __any_sync(0xffffffffu, from > 0);
+      f2 pr[32];
+      uint32_t word[32];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float4 l = lds4(rows + e * 16);
+        const uint32_t* x = &s[e >> 3][(e & 7) * 4];
+        const f2 a = f2_fma(f2_make(__uint_as_float(x[0]), __uint_as_float(x[1])), c2, f2_mul(f2_make(l.x, l.y), minus));
+        const f2 d = f2_fma(f2_make(__uint_as_float(x[2]), __uint_as_float(x[3])), c2, f2_mul(f2_make(l.z, l.w), minus));
+        float y0 = exp2_approx(f2_lo(a)), y1 = exp2_approx(f2_hi(a)), y2 = exp2_approx(f2_lo(d)), y3 = exp2_approx(f2_hi(d));
+        if (edge) {
+          y0 = 4 * e >= from ? y0 : 0.f;
+          y1 = 4 * e + 1 >= from ? y1 : 0.f;
+          y2 = 4 * e + 2 >= from ? y2 : 0.f;
+          y3 = 4 * e + 3 >= from ? y3 : 0.f;
+        }
+        pr[2 * e] = f2_make(y0, y1);
+        pr[2 * e + 1] = f2_make(y2, y3);
+        word[2 * e] = bf16_of_f2(pr[2 * e]);
+        word[2 * e + 1] = bf16_of_f2(pr[2 * e + 1]);
+      }
+      tc_st32(s_at, word);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(m.bar(kPReady));
+
+      ok = warp_wait(m.bar(kDpFull), i & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      tc_ld32(dp_at, s[0]);
+      tc_ld32(dp_at + 32, s[1]);
+      tc_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float4 l = lds4(rows + kTile * 4 + e * 16);
+        const uint32_t* x = &s[e >> 3][(e & 7) * 4];
+        f2 a = f2_mul(pr[2 * e], f2_fma(f2_make(l.x, l.y), minus, f2_make(__uint_as_float(x[0]), __uint_as_float(x[1]))));
+        f2 d = f2_mul(pr[2 * e + 1], f2_fma(f2_make(l.z, l.w), minus, f2_make(__uint_as_float(x[2]), __uint_as_float(x[3]))));
+        if (!row_ok) a = d = 0ull;        // what lies behind the sample's keys may be NaN
+        word[2 * e] = bf16_of_f2(a);
+        word[2 * e + 1] = bf16_of_f2(d);
+      }
+      tc_st32(dp_at, word);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(m.bar(kDsReady));
+    }
+    if (ok && count > 0) {
+      ok = warp_wait(m.bar(kDone), 0, &abort_flag);
+      tc_fence_after();
+    }
+    const int64_t at = ((static_cast<int64_t>(b) * z.lk + row) * z.kv_heads + hk) * D;
+    __nv_bfloat16* dst = w == 0 ? p.dv : p.dk;
+    float* part = w == 0 ? p.part0 : p.part1;
+    store_row<D>(tmem + lanes + (w == 0 ? C::kAcc0 : C::kAcc1), count > 0, w == 0 ? 1.f : p.scale, ok && row < z.lk,
+                 dst ? dst + at : nullptr, part ? part + split * p.elements + at : nullptr);
+  }
+  teardown(&abort_flag, p.status, tmem, warp);
+}
+
+// ------------------------------------------------------------------------------------------------ queries: dQ
+// grid (query tiles * splits, heads, batch). P stays in registers here, so the scores have two buffers and S(j + 1) is ready
+// when the warpgroups come to it.
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                             const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                             const __grid_constant__ BwdParams p) {
+  using C = BwdCfg<D>;
+  constexpr uint32_t kBytes = tile_bytes<D>();
+  constexpr uint32_t kS1 = C::kAcc1;       // second buffer of the scores: 256 + D .. 384 + D
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ volatile int abort_flag;
+  __shared__ uint32_t tmem_slot;
+  const Layout<D> m{(smem_u32(smem_raw) + 1023u) & ~1023u};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  setup<D>(m, &abort_flag, &tmem_slot, warp);
+  const uint32_t tmem = tmem_slot;
+
+  const Sizes& z = p.z;
+  const int split = blockIdx.x % p.splits, qt = blockIdx.x / p.splits, h = blockIdx.y, b = blockIdx.z;
+  const int hk = h / z.group, q0 = qt * kTile, n = keys_of(z, b);
+  const int lim_tile = key_limit(z, n, min(z.lq, q0 + kTile) - 1);
+  const int j0 = split * p.per_split, count = max(0, min((lim_tile + kTile - 1) / kTile, j0 + p.per_split) - j0);
+
+  if (warp == 9) {
+    // ------------------------------------------------------------ TMA producer: K0, V0, K1, V1, ...
+    if (lane == 0 && count > 0) {
+      mbar_expect_tx(m.bar(kFixedFull), 2 * kBytes);
+      load_tile<D>(m.fixed(0), &map_q, m.bar(kFixedFull), q0, h, b);
+      load_tile<D>(m.fixed(1), &map_do, m.bar(kFixedFull), q0, h, b);
+      for (int i = 0; i < 2 * count; ++i) {
+        const int s = i % C::kStages;
+        if (!mbar_wait(m.empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
+        mbar_expect_tx(m.full(s), kBytes);
+        load_tile<D>(m.stage(s), (i & 1) ? &map_v : &map_k, m.full(s), (j0 + (i >> 1)) * kTile, hk, b);
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA issuer
+    auto wait_stage = [&](int i) { return warp_wait(m.full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
+    auto steps_of = [&](int j) { return (min(kTile, n - (j0 + j) * kTile) + 15) / 16; };
+    auto scores = [&](int j) {             // S(j) = Q K_j^T; the keys' rows behind the sample's length are cleared for dS K
+      if (!wait_stage(2 * j)) return false;
+      const int keys = min(kTile, n - (j0 + j) * kTile);
+      if (keys & 15) zero_rows<D>(m.stage(2 * j % C::kStages), keys, steps_of(j) * 16);
+      tc_fence_after();
+      if (lane == 0) {
+        product_ss<D>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(2 * j % C::kStages));
+        tc_commit(m.bar(kSFull + (j & 1)));
+      }
+      __syncwarp();
+      return true;
+    };
+    auto gradients = [&](int j) {          // dP(j) = dO V_j^T
+      if (!wait_stage(2 * j + 1)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage((2 * j + 1) % C::kStages));
+        tc_commit(m.bar(kDpFull));
+        tc_commit(m.empty((2 * j + 1) % C::kStages));
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0) && (count == 1 || scores(1));
+    for (int j = 0; j < count && ok; ++j) {
+      ok = warp_wait(m.bar(kDsReady), j & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      if (lane == 0) {
+        product_ts<D>(tmem + C::kAcc0, tmem + C::kDp, m.stage(2 * j % C::kStages), steps_of(j), j > 0);
+        tc_commit(j + 1 < count ? m.empty(2 * j % C::kStages) : m.bar(kDone));
+      }
+      __syncwarp();
+      if (j + 1 < count) ok = gradients(j + 1);
+      if (ok && j + 2 < count) ok = scores(j + 2);
+    }
+  } else {
+    // ------------------------------------------------------------ probabilities: thread = query, warpgroup w has 64 keys
+    const int w = warp >> 2, row = q0 + (threadIdx.x & 127);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t dp_at = tmem + lanes + C::kDp + w * 64;
+    const int lim = key_limit(z, n, row);
+    const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
+    const int64_t r = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + row;
+    const f2 c2 = f2_dup(p.c), lse = f2_dup(-p.lse2[r]), delta = f2_dup(-p.delta[r]);
+    bool ok = true;
+    for (int j = 0; j < count; ++j) {
+      ok = warp_wait(m.bar(kSFull + (j & 1)), (j >> 1) & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t s_at = tmem + lanes + ((j & 1) ? kS1 : C::kS) + w * 64;
+      uint32_t s[2][32];
+      tc_ld32(s_at, s[0]);
+      tc_ld32(s_at + 32, s[1]);
+      tc_wait_ld();
+      const int k0 = (j0 + j) * kTile + w * 64;
+      const bool edge = k0 + 64 > lim_all;
+      f2 pr[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const uint32_t* x = &s[e >> 4][(e & 15) * 2];
+        const f2 a = f2_fma(f2_make(__uint_as_float(x[0]), __uint_as_float(x[1])), c2, lse);
+        float y0 = exp2_approx(f2_lo(a)), y1 = exp2_approx(f2_hi(a));
+        if (edge) {
+          y0 = k0 + 2 * e < lim ? y0 : 0.f;
+          y1 = k0 + 2 * e + 1 < lim ? y1 : 0.f;
+        }
+        pr[e] = f2_make(y0, y1);
+      }
+      ok = warp_wait(m.bar(kDpFull), j & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      tc_ld32(dp_at, s[0]);
+      tc_ld32(dp_at + 32, s[1]);
+      tc_wait_ld();
+      uint32_t word[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const uint32_t* x = &s[e >> 4][(e & 15) * 2];
+        const f2 a = f2_mul(pr[e], f2_add(f2_make(__uint_as_float(x[0]), __uint_as_float(x[1])), delta));
+        float y0 = f2_lo(a), y1 = f2_hi(a);
+        if (edge) {                        // what lies behind the sample's keys may be NaN
+          y0 = k0 + 2 * e < lim ? y0 : 0.f;
+          y1 = k0 + 2 * e + 1 < lim ? y1 : 0.f;
+        }
+        word[e] = bf16_of_f2(f2_make(y0, y1));
+      }
+      tc_st32(dp_at, word);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(m.bar(kDsReady));
+    }
+    if (ok && count > 0) {
+      ok = warp_wait(m.bar(kDone), 0, &abort_flag);
+      tc_fence_after();
+    }
+    if (w == 0) {
+      const int64_t dense = ((static_cast<int64_t>(b) * z.heads + h) * z.lq + row) * D;
+      store_row<D>(tmem + lanes + C::kAcc0, count > 0, p.scale, ok && row < z.lq,
+                   p.dq + b * p.sdq.b + row * p.sdq.l + h * p.sdq.h, p.part0 ? p.part0 + split * p.elements + dense : nullptr);
+    }
+  }
+  teardown(&abort_flag, p.status, tmem, warp);
+}
+
+// ------------------------------------------------------------------------------------------------ joining the ranges
+// dst[row] = sum over splits of part[split][row] in ascending order; rows of D, one of (batch, head, token) order for dq. Four
+// elements a thread.
+struct SumParams {
+  const float* part;
+  __nv_bfloat16* dst;
+  int splits;
+  int64_t elements;
+  int d, lq, heads;                      // lq > 0: rows are (batch, head, token), dst has strides
+  Strided s;
+};
+__global__ void __launch_bounds__(256) attention_sum_kernel(const __grid_constant__ SumParams p) {
+  after_previous();
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= p.elements) return;
+  const float* src = after_previous(p.part) + i;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(src + s * p.elements);
+    t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+  }
+  __nv_bfloat16* dst = p.dst + i;
+  if (p.lq) {
+    const int64_t row = i / p.d, bh = row / p.lq, l = row - bh * p.lq, b = bh / p.heads, h = bh - b * p.heads;
+    dst = p.dst + b * p.s.b + l * p.s.l + h * p.s.h + (i - row * p.d);
+  }
+  __nv_bfloat162 o[2] = {__floats2bfloat162_rn(t.x, t.y), __floats2bfloat162_rn(t.z, t.w)};
+  *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+}
+
+// Ranges the work of `ctas` CTAs, `items` passes each, is cut into: two CTAs a SM, none with fewer than four passes; one where
+// there are CTAs enough.
+int split_count(int64_t ctas, int64_t items) {
+  if (ctas == 0 || ctas >= sm_count()) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(2LL * sm_count(), ctas), items / 4)));
+}
+struct Plan {
+  int64_t lq_pad, row_floats;            // lse2 and delta
+  int key_splits, key_per, query_splits, query_per;
+  int64_t key_elements, query_elements;
+  Plan(const Shape& s, bool want_keys, bool want_queries) {
+    const int64_t q_tiles = ceil_div(s.lq, kTile), k_tiles = ceil_div(s.lk, kTile), group = s.heads / s.kv_heads;
+    lq_pad = q_tiles * kTile;
+    row_floats = 2 * s.batch * s.heads * lq_pad;
+    key_splits = want_keys ? split_count(k_tiles * s.kv_heads * s.batch, group * q_tiles) : 1;
+    key_per = static_cast<int>(std::max<int64_t>(1, ceil_div(group * q_tiles, key_splits)));
+    query_splits = want_queries ? split_count(q_tiles * s.heads * s.batch, k_tiles) : 1;
+    query_per = static_cast<int>(std::max<int64_t>(1, ceil_div(k_tiles, query_splits)));
+    key_elements = s.batch * s.lk * s.kv_heads * s.d;
+    query_elements = s.batch * s.lq * s.heads * s.d;
+  }
+  // the partial sums of the keys are read before those of the queries are written: one buffer
+  int64_t part_floats() const {
+    return std::max(key_splits > 1 ? 2 * key_splits * key_elements : 0, query_splits > 1 ? query_splits * query_elements : 0);
+  }
+  int64_t bytes() const { return (row_floats + part_floats()) * 4; }
+};
+
+template <int D>
+int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Shape& s, const RowsParams& rows, BwdParams p, cudaStream_t st) {
+  using C = BwdCfg<D>;
+  static PerDeviceOnce once;
+  const cudaError_t rc = per_device_once(once, [] {
+    cudaError_t e = cudaFuncSetAttribute(attention_bwd_keys_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    return e ? e : cudaFuncSetAttribute(attention_bwd_queries_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  });
+  ANIMA_REQUIRE(rc == cudaSuccess, ANIMA_E_CUDA, "%s: cannot reserve %d bytes of shared memory: %s", who, C::kSmem,
+                cudaGetErrorString(rc));
+  float* part = p.part0;
+  if (rows.rows) {
+    launch_after(attention_rows_kernel<D>, dim3(static_cast<unsigned>(ceil_div(rows.rows, 256 / (D / 8)))), dim3(256), 0, st, rows);
+    ANIMA_CHECK_LAUNCH(who);
+  }
+  auto join = [&](const float* from, __nv_bfloat16* to, int splits, int64_t elements, int lq) {
+    const SumParams sp = {from, to, splits, elements, D, lq, p.z.heads, p.sdq};
+    launch_after(attention_sum_kernel, dim3(static_cast<unsigned>(ceil_div(elements, 1024))), dim3(256), 0, st, sp);
+    ANIMA_CHECK_LAUNCH(who);
+    return ANIMA_OK;
+  };
+  if ((p.dk || p.dv) && plan.key_elements) {
+    p.splits = plan.key_splits;
+    p.per_split = plan.key_per;
+    p.elements = plan.key_elements;
+    p.part0 = p.splits > 1 ? part : nullptr;
+    p.part1 = p.splits > 1 ? part + p.splits * p.elements : nullptr;
+    const dim3 grid(static_cast<unsigned>(ceil_div(s.lk, kTile) * p.splits), static_cast<unsigned>(s.kv_heads), static_cast<unsigned>(s.batch));
+    launch_after(attention_bwd_keys_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
+    ANIMA_CHECK_LAUNCH(who);
+    if (p.splits > 1) {
+      if (p.dv)
+        if (int e = join(p.part0, p.dv, p.splits, p.elements, 0)) return e;
+      if (p.dk)
+        if (int e = join(p.part1, p.dk, p.splits, p.elements, 0)) return e;
+    }
+  }
+  if (p.dq && plan.query_elements) {
+    p.splits = plan.query_splits;
+    p.per_split = plan.query_per;
+    p.elements = plan.query_elements;
+    p.part0 = p.splits > 1 ? part : nullptr;
+    const dim3 grid(static_cast<unsigned>(ceil_div(s.lq, kTile) * p.splits), static_cast<unsigned>(s.heads), static_cast<unsigned>(s.batch));
+    launch_after(attention_bwd_queries_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
+    ANIMA_CHECK_LAUNCH(who);
+    if (p.splits > 1) return join(p.part0, p.dq, p.splits, p.elements, p.z.lq);
+  }
   return ANIMA_OK;
 }
-int check_tensor(const char* who, const char* name, const void* p, const int64_t* s, bool empty) {
-  ANIMA_REQUIRE(s, ANIMA_E_ARG, "%s: strides of %s are missing", who, name);
-  ANIMA_REQUIRE(p || empty, ANIMA_E_ARG, "%s: null pointer (%s)", who, name);
-  ANIMA_REQUIRE(s[0] >= 0 && s[1] >= 0 && s[2] >= 0, ANIMA_E_ARG, "%s: negative stride of %s", who, name);
-  ANIMA_REQUIRE(aligned16(p) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0, ANIMA_E_ALIGN,
-                "%s: %s must be 16-byte aligned, its strides multiples of 8 elements", who, name);
-  return ANIMA_OK;
-}
-Strided strided(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
 }  // namespace
+}  // namespace attn
 }  // namespace anima
 
 using namespace anima;
 
 extern "C" int64_t anima_attention_bwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
                                                        int64_t head_dim, int causal) {
-  (void)causal;
-  if (int rc = check_sizes("attention_bwd", batch, lq, lk, heads, kv_heads, head_dim)) return rc;
-  return batch * heads * lq * 4;
+  if (int rc = attn::check_sizes("attention_bwd", batch, lq, lk, heads, kv_heads, head_dim)) return rc;
+  return attn::Plan(attn::Shape(batch, lq, lk, heads, kv_heads, head_dim, causal), true, true).bytes();
 }
 
 extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides,
@@ -156,50 +651,60 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
                                    void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes, int32_t* status,
                                    void* stream) {
   const char* who = "attention_bwd";
-  (void)status;
   const int64_t need = anima_attention_bwd_workspace_bytes(batch, lq, lk, heads, kv_heads, head_dim, causal);
-  if (need < 0) return (int)need;
+  if (need < 0) return static_cast<int>(need);
   ANIMA_REQUIRE(scale > 0.f && scale < INFINITY, ANIMA_E_ARG, "%s: scale must be positive and finite", who);
   const bool no_q = batch * lq == 0, no_k = batch * lk == 0;
-  if (int rc = check_tensor(who, "dout", dout, dout_strides, no_q)) return rc;
-  if (int rc = check_tensor(who, "q", q, q_strides, no_q)) return rc;
-  if (int rc = check_tensor(who, "k", k, k_strides, no_k)) return rc;
-  if (int rc = check_tensor(who, "v", v, v_strides, no_k)) return rc;
+  if (int rc = attn::check_tensor(who, "dout", dout, dout_strides, no_q)) return rc;
+  if (int rc = attn::check_tensor(who, "q", q, q_strides, no_q)) return rc;
+  if (int rc = attn::check_tensor(who, "k", k, k_strides, no_k)) return rc;
+  if (int rc = attn::check_tensor(who, "v", v, v_strides, no_k)) return rc;
   ANIMA_REQUIRE(no_q || (out && lse), ANIMA_E_ARG, "%s: null pointer", who);
   ANIMA_REQUIRE(aligned16(out) && aligned16(dq) && aligned16(dk) && aligned16(dv) && aligned16(workspace), ANIMA_E_ALIGN,
                 "%s: tensors must be 16-byte aligned", who);
   ANIMA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), ANIMA_E_WORKSPACE, "%s: workspace of %lld bytes, %lld needed",
                 who, (long long)workspace_bytes, (long long)need);
-  AttnParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
-  p.v = static_cast<const __nv_bfloat16*>(v);
-  p.out = static_cast<const __nv_bfloat16*>(out);
-  p.dout = static_cast<const __nv_bfloat16*>(dout);
-  p.sq = strided(q_strides);
-  p.sk = strided(k_strides);
-  p.sv = strided(v_strides);
-  p.sdo = strided(dout_strides);
-  p.lengths = kv_lengths;
-  p.lq = (int)lq; p.lk = (int)lk; p.heads = (int)heads; p.kv_heads = (int)kv_heads; p.causal = causal;
+  if (no_q && no_k) return ANIMA_OK;
+  const attn::Shape s(batch, lq, lk, heads, kv_heads, head_dim, causal);
+  const attn::Plan plan(s, dk || dv, dq != nullptr);
+  attn::Strided sq = attn::strided(q_strides), sdo = attn::strided(dout_strides);
+  attn::Strided dense = {lq * heads * head_dim, heads * head_dim, head_dim};
+  s.regroup(sq);
+  s.regroup(sdo);
+  s.regroup(dense);
+  float* ws = static_cast<float*>(workspace);
+  attn::BwdParams p = {};
+  p.z = s.sizes(kv_lengths);
+  p.c = scale * attn::kLog2e;
   p.scale = scale;
-  p.lse = const_cast<float*>(lse);
-  p.delta = static_cast<float*>(workspace);
+  p.lse2 = ws;
+  p.delta = ws + plan.row_floats / 2;
+  p.lq_pad = static_cast<int>(plan.lq_pad);
   p.dq = static_cast<__nv_bfloat16*>(dq);
   p.dk = static_cast<__nv_bfloat16*>(dk);
   p.dv = static_cast<__nv_bfloat16*>(dv);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (!no_q) {
-    const dim3 grid((unsigned)ceil_div(lq, kWarps), (unsigned)heads, (unsigned)batch);
-    if (head_dim == 64) attention_rows_kernel<64><<<grid, kWarps * 32, 0, s>>>(p);
-    else attention_rows_kernel<128><<<grid, kWarps * 32, 0, s>>>(p);
-    ANIMA_CHECK_LAUNCH(who);
-  }
-  if (!no_k && (dk || dv)) {
-    const dim3 grid((unsigned)ceil_div(lk, kWarps), (unsigned)kv_heads, (unsigned)batch);
-    if (head_dim == 64) attention_keys_kernel<64><<<grid, kWarps * 32, 0, s>>>(p);
-    else attention_keys_kernel<128><<<grid, kWarps * 32, 0, s>>>(p);
-    ANIMA_CHECK_LAUNCH(who);
-  }
-  return ANIMA_OK;
+  p.sdq = dense;
+  p.part0 = ws + plan.row_floats;
+  p.status = status;
+  attn::RowsParams rows = {};
+  rows.out = static_cast<const __nv_bfloat16*>(out);
+  rows.dout = static_cast<const __nv_bfloat16*>(dout);
+  rows.so = dense;
+  rows.sdo = sdo;
+  rows.lse = lse;
+  rows.lse2 = ws;
+  rows.delta = ws + plan.row_floats / 2;
+  rows.lq = p.z.lq;
+  rows.lq_pad = p.lq_pad;
+  rows.heads = p.z.heads;
+  rows.rows = s.batch * plan.lq_pad * s.heads;
+  const void* stand_in = no_q ? k : q;
+  CUtensorMap maps[4];
+  ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, stand_in) &&
+                    attn::encode_heads(&maps[1], dout, sdo, s.batch, s.lq, s.heads, s.d, stand_in) &&
+                    attn::encode_heads(&maps[2], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in) &&
+                    attn::encode_heads(&maps[3], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in),
+                ANIMA_E_CUDA, "%s: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand)", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return head_dim == 64 ? attn::launch<64>(who, maps, plan, s, rows, p, st) : attn::launch<128>(who, maps, plan, s, rows, p, st);
 }

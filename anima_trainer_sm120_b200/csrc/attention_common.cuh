@@ -103,6 +103,33 @@ inline int check_tensor(const char* who, const char* name, const void* p, const 
 }
 inline Strided strided(const int64_t* s) { return {s[0], s[1], s[2]}; }
 
+// Sizes of a call as the kernels see it. One query token a sample: the heads that share a key head become its tokens (all
+// keys of the sample are seen, so nothing depends on a query's place), and each key is read once for all of them.
+struct Shape {
+  int64_t batch, lq, lk, heads, kv_heads, d;
+  int causal;
+  bool regrouped;
+  Shape(int64_t batch, int64_t lq_, int64_t lk, int64_t heads_, int64_t kv_heads, int64_t d, int causal_)
+      : batch(batch), lq(lq_ == 1 ? heads_ / kv_heads : lq_), lk(lk), heads(lq_ == 1 ? kv_heads : heads_), kv_heads(kv_heads), d(d),
+        causal(lq_ == 1 ? 0 : causal_ != 0), regrouped(lq_ == 1) {}
+  void regroup(Strided& s) const {       // of a tensor with the queries' heads
+    if (!regrouped) return;
+    s.l = s.h;
+    s.h = s.l * lq;
+  }
+  Sizes sizes(const int32_t* lengths) const {
+    return {static_cast<int>(lq), static_cast<int>(lk), static_cast<int>(heads), static_cast<int>(kv_heads),
+            static_cast<int>(heads / kv_heads), causal, lengths};
+  }
+};
+
+// A thread that has made no runtime call yet (autograd's worker, say) has no current context, without which the driver
+// refuses to encode a tensor map; making its device current again binds one.
+inline bool bind_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
 // Tensor map of a (batch, token, head, D) bf16 tensor, boxes of 128 tokens x 64 elements. A tensor without elements gets the
 // map of one that is never read (`stand_in`: any valid address).
 inline bool encode_heads(CUtensorMap* map, const void* p, const Strided& s, int64_t batch, int64_t len, int64_t heads, int64_t d,

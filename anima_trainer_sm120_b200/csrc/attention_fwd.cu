@@ -353,22 +353,6 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
   if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + log2_approx(l)) * kLn2;
 }
 
-// One query token a sample: the heads of a group become its tokens (nothing of the computation depends on a query's place: all
-// keys of the sample are seen).
-struct Shape {
-  int64_t batch, lq, lk, heads, kv_heads, d;
-  int causal;
-  bool regrouped = false;
-  Shape(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d, int causal)
-      : batch(batch), lq(lq), lk(lk), heads(heads), kv_heads(kv_heads), d(d), causal(causal) {
-    if (lq != 1) return;
-    this->causal = 0;
-    this->lq = heads / kv_heads;
-    this->heads = kv_heads;
-    regrouped = true;
-  }
-};
-
 // Ranges the keys are cut into: as many as give every SM two CTAs, none shorter than four tiles.
 int split_count(const Shape& s) {
   const int64_t ctas = ceil_div(s.lq, 2 * kTile) * s.heads * s.batch, tiles = ceil_div(s.lk, kTile);
@@ -430,14 +414,9 @@ extern "C" int anima_attention_fwd(const void* q, const int64_t* q_strides, cons
   attn::Strided sq = attn::strided(q_strides);
   attn::FwdParams p = {};
   p.so = {lq * heads * head_dim, heads * head_dim, head_dim};
-  if (s.regrouped) {
-    sq.l = sq.h;
-    sq.h = sq.l * s.lq;
-    p.so.l = head_dim;
-    p.so.h = head_dim * s.lq;
-  }
-  p.z = {static_cast<int>(s.lq), static_cast<int>(s.lk), static_cast<int>(s.heads), static_cast<int>(s.kv_heads),
-         static_cast<int>(s.heads / s.kv_heads), s.causal, kv_lengths};
+  s.regroup(sq);
+  s.regroup(p.so);
+  p.z = s.sizes(kv_lengths);
   p.c = scale * attn::kLog2e;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
@@ -451,7 +430,7 @@ extern "C" int anima_attention_fwd(const void* q, const int64_t* q_strides, cons
     p.part_lse = p.part_o + p.splits * p.rows * head_dim;
   }
   CUtensorMap maps[3];
-  ANIMA_REQUIRE(attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, q) &&
+  ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, q) &&
                     attn::encode_heads(&maps[1], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, q) &&
                     attn::encode_heads(&maps[2], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, q),
                 ANIMA_E_CUDA, "%s: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand)", who);

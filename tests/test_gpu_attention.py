@@ -90,6 +90,21 @@ def test_causal_with_more_queries_than_keys_leaves_the_first_rows_empty():
     assert not out[:, :160].any() and not dq[:, :160].any() and bool((lse[:, :, :160] == -float("inf")).all())
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_empty_rows_hold_has_no_part_in_anything(D):
+    """Causal, more queries than keys, NaN in q and in the incoming gradient of the queries that see no key."""
+    from anima_trainer_sm120_b200.attention_kernel import fused_attention
+    q, k, v, g = _tensors(1, 500, 190, 4, 2, D, seed=15)
+    results = []
+    for bad in (0.0, float("nan")):
+        q[:, :310] = bad
+        g[:, :310] = bad
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        out = fused_attention(*leaves, causal=True)
+        results.append([out.detach(), *torch.autograd.grad(out, leaves, g)])
+    assert all(bool(torch.isfinite(b).all()) and torch.equal(a, b) for a, b in zip(*results))
+
+
 @pytest.mark.parametrize("lengths", [[2 ** 31 - 1, -5], [400, 0]])
 def test_lengths_outside_the_keys_are_clamped(lengths):
     q, k, v, g = _tensors(2, 70, 100, 2, 2, 64, seed=3)
@@ -288,6 +303,27 @@ def test_another_stream_and_two_calls_at_once():
     torch.cuda.synchronize()
     for w, o in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(w, o))
+
+
+def test_first_call_of_a_new_thread():
+    """A thread without a current context: the caller's own, and autograd's worker."""
+    import threading
+    from anima_trainer_sm120_b200.attention_kernel import fused_attention
+    q, k, v, g = _tensors(1, 40, 60, 2, 2, 64, seed=5)
+    found = []
+
+    def go():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        out = fused_attention(*leaves)
+        found.append([out.detach(), *torch.autograd.grad(out, leaves, g)])
+
+    for _ in range(2):
+        t = threading.Thread(target=go)
+        t.start()
+        t.join()
+    go()
+    torch.cuda.synchronize()
+    assert len(found) == 3 and all(torch.equal(a, b) for f in found[:2] for a, b in zip(f, found[2]))
 
 
 def test_captured_and_replayed_with_other_inputs():
