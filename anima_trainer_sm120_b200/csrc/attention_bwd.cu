@@ -1,8 +1,8 @@
 // Attention, backward (formulas: attention_common.cuh): the probabilities are made again from q, k and the forward's log-sums.
 //
 // Three launches, no atomics, every sum in a fixed order:
-//   rows   delta = out . dout of each query, and its log-sum in base 2 (+inf for a query that saw nothing, and for the rows that
-//          fill up the last tile: their probabilities come out as 0);
+//   rows   -delta = -out . dout of each query, and minus its log-sum in base 2 (-inf for a query that saw nothing, and for the
+//          rows that fill up the last tile: their probabilities come out as 0);
 //   keys   one CTA a tile of 128 keys of a key head walks the query tiles of all heads it serves:
 //            S^T = K Q^T, dP^T = V dO^T (lane = key, column = query), dV += P^T dO, dK += dS^T Q;
 //   queries one CTA a tile of 128 queries of a head walks the key tiles:
@@ -13,9 +13,9 @@
 // whose order would change results, and 4 bytes a key tile and element of traffic), and the sums stay in tensor memory.
 // Each tile of q, dO, K lies in shared memory once and serves as a K-major operand of one product and as an MN-major operand
 // of another.
-// Two warpgroups share a tile pair, 64 columns each; warp 8 issues the products so that the tensor cores work on the ones
-// that are ready while the warpgroups make the next probabilities: dV(i) and S(i+1) as soon as P(i) lies in tensor memory,
-// dK(i) and dP(i+1) as soon as dS(i) does.
+// A query tile (keys kernel) or key tile (queries kernel) is taken in two halves of 64, each with tensor memory, barriers and two
+// of the four warpgroups of its own: while one half makes exponentials, the other makes dS, and the tensor cores work on what
+// either has finished. One warp issues all products, in the order in which the halves get ready.
 // Bound: 14 D flop a (query, key) pair on the tensor cores; two exponentials.
 #include "attention_common.cuh"
 
@@ -23,12 +23,15 @@ namespace anima {
 namespace attn {
 namespace {
 
-constexpr int kThreads = 320;            // two warpgroups, one MMA warp, one TMA warp
+constexpr int kWorkers = 16;             // warps that make probabilities: two warpgroups for each half of a tile
+constexpr int kMmaWarp = kWorkers, kTmaWarp = kWorkers + 1, kThreads = (kWorkers + 2) * 32;
+constexpr int kHalf = kTile / 2;
+constexpr int kPoly = 0;                 // of four pairs of exponentials, those made on the multiply-add pipes
 
 struct BwdParams {
   Sizes z;
   float c, scale;                        // scale * log2 e, scale
-  const float *lse2, *delta;             // [batch, heads, lq_pad]
+  const float *lse2, *delta;             // [batch, heads, lq_pad], both negated
   int lq_pad;
   __nv_bfloat16 *dq, *dk, *dv;
   Strided sdq;                           // dk, dv: dense
@@ -71,47 +74,53 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
   for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(((1ull << kLanes) - 1) << (threadIdx.x & 31 & ~(kLanes - 1)), s, o);
   if (lane != 0) return;
   const float lse = l < p.lq ? after_previous(p.lse)[(b * p.heads + h) * p.lq + l] : -INFINITY;
-  p.lse2[to] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-  p.delta[to] = lse == -INFINITY ? 0.f : s;
+  p.lse2[to] = lse == -INFINITY ? -INFINITY : lse * -kLog2e;
+  p.delta[to] = lse == -INFINITY ? 0.f : -s;
 }
 
+// Shared memory: two tiles that stay, a ring (keys: half tiles of q with their lse2 and delta, and of dout; queries: tiles of K
+// and V), barriers.
 template <int D>
 struct BwdCfg {
-  static constexpr int kStages = D == 128 ? 4 : 8;                     // tiles in flight beside the two that stay
-  static constexpr int kBars = 2 * kStages + 8;
-  static constexpr int kRowBytes = 2 * kTile * 4;                      // lse2 and delta of a query tile
-  static constexpr int kSmem = (2 + kStages) * static_cast<int>(tile_bytes<D>()) + kStages / 2 * kRowBytes + 1024 + kBars * 8 + 16;
+  static constexpr uint32_t kBytes = tile_bytes<D>(), kHalfBytes = kBytes / 2;
+  static constexpr int kSlots = 5;                                     // half tiles of q, and of dout
+  static constexpr int kRowBytes = 2 * kHalf * 4;                      // lse2 and delta of a half
+  static constexpr int kStages = 5;                                    // tiles of K or V
+  static constexpr int kBars = 4 * kSlots + 12;
+  static constexpr int kSmem = 2 * kBytes + kSlots * (2 * kHalfBytes + kRowBytes) + kBars * 8;
+  static_assert(kSlots * 2 * kHalfBytes >= kStages * kBytes, "one size for both kernels");
+  static_assert(kSmem <= 227 * 1024, "shared memory");
   static constexpr uint32_t kS = 0, kDp = 128, kAcc0 = 256, kAcc1 = 256 + D;   // tensor-memory columns
 };
-
-// Shared memory and barriers of either kernel.
 template <int D>
 struct Layout {
   using C = BwdCfg<D>;
   uint32_t base;
-  __device__ __forceinline__ uint32_t fixed(int i) const { return base + i * tile_bytes<D>(); }
-  __device__ __forceinline__ uint32_t stage(int s) const { return base + (2 + s) * tile_bytes<D>(); }
-  __device__ __forceinline__ uint32_t row_data(int s) const { return base + (2 + C::kStages) * tile_bytes<D>() + (s >> 1) * C::kRowBytes; }
-  __device__ __forceinline__ uint32_t bars() const { return base + (2 + C::kStages) * tile_bytes<D>() + C::kStages / 2 * C::kRowBytes; }
-  __device__ __forceinline__ uint32_t full(int s) const { return bars() + 8 * s; }
-  __device__ __forceinline__ uint32_t empty(int s) const { return bars() + 8 * (C::kStages + s); }
-  __device__ __forceinline__ uint32_t bar(int i) const { return bars() + 8 * (2 * C::kStages + i); }
+  __device__ __forceinline__ uint32_t fixed(int i) const { return base + i * C::kBytes; }
+  __device__ __forceinline__ uint32_t ring() const { return base + 2 * C::kBytes; }
+  __device__ __forceinline__ uint32_t stage(int s) const { return ring() + s * C::kBytes; }                            // queries
+  __device__ __forceinline__ uint32_t q(int s) const { return ring() + s * C::kHalfBytes; }                            // keys
+  __device__ __forceinline__ uint32_t g(int s) const { return ring() + (C::kSlots + s) * C::kHalfBytes; }
+  __device__ __forceinline__ uint32_t row_data(int s) const { return ring() + 2 * C::kSlots * C::kHalfBytes + s * C::kRowBytes; }
+  __device__ __forceinline__ uint32_t bar(int i) const { return row_data(C::kSlots) + 8 * i; }     // 10, 11: the abort flag, the tensor-memory address
+  __device__ __forceinline__ uint32_t full(int s) const { return bar(12 + s); }
+  __device__ __forceinline__ uint32_t empty(int s) const { return bar(12 + C::kSlots + s); }
+  __device__ __forceinline__ uint32_t full2(int s) const { return bar(12 + 2 * C::kSlots + s); }
+  __device__ __forceinline__ uint32_t empty2(int s) const { return bar(12 + 3 * C::kSlots + s); }
 };
-enum { kFixedFull, kSFull, kSFull1, kDpFull, kPReady, kDsReady, kDone };
+// one barrier each, or one for each half (or score buffer)
+enum { kFixedFull = 0, kDone = 1, kSFull = 2, kDpFull = 4, kPReady = 6, kDsReady = 8 };
 
 template <int D>
 __device__ __forceinline__ void setup(const Layout<D>& m, volatile int* abort_flag, uint32_t* tmem_slot, int warp) {
   using C = BwdCfg<D>;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(m.full(s), 1);
-      mbar_init(m.empty(s), 1);
-    }
-    for (int i = kFixedFull; i <= kDone; ++i) mbar_init(m.bar(i), i == kPReady || i == kDsReady ? 8 : 1);
+    for (int i = 0; i < C::kBars; ++i)
+      if (i < 10 || i >= 12) mbar_init(m.bar(i), i >= kPReady && i < kDsReady + 2 ? kWorkers / 2 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) tc_alloc(smem_u32(tmem_slot), 512);
+  if (warp == kMmaWarp) tc_alloc(smem_u32(tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -126,68 +135,70 @@ __device__ __forceinline__ void teardown(volatile int* abort_flag, int32_t* stat
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tc_dealloc(tmem, 512);
   }
 }
 
-// D[tmem] (+)= A . B^T, both tiles in shared memory with the head vector along K
-template <int D>
-__device__ __forceinline__ void product_ss(uint32_t d, uint32_t a_smem, uint32_t b_smem) {
+// D[tmem] = A . B^T: A a tile of 128 rows, B of N rows whose 64-column chunks lie b_chunk bytes apart, the head vector along K
+template <int D, int N>
+__device__ __forceinline__ void product_ss(uint32_t d, uint32_t a_smem, uint32_t b_smem, uint32_t b_chunk) {
   const uint64_t a = tc_desc_sw128(a_smem), b = tc_desc_sw128(b_smem);
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) {
-    const uint32_t at = (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2;     // 16 bytes a unit
-    tc_mma_ss(d, a + at, b + at, tc_idesc_bf16(kTile, kTile), i > 0);
-  }
+  for (int i = 0; i < D / 16; ++i)      // 16 bytes a unit
+    tc_mma_ss(d, a + (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2, b + (i >> 2) * (b_chunk / 16) + (i & 3) * 2, tc_idesc_bf16(kTile, N), i > 0);
 }
-// D[tmem] += A . B: A [128, 16 steps] bf16 in tensor memory, columns 0-63 at `a`, 64-127 at a + 64; B a tile with its rows along K
+// D[tmem] += A . B over 16 `steps` (at most 4) rows of B (64-column chunks b_chunk bytes apart): A bf16 in tensor memory, elements 32 w .. 32 w + 31
+// of a row in columns a + 32 w .. + 15
 template <int D>
-__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b_smem, int steps, bool accumulate) {
-  const uint64_t b = tc_desc_sw128(b_smem, kTile * 128);
-  for (int i = 0; i < steps; ++i)
-    tc_mma_ts(d, a + (i >> 2) * 64 + (i & 3) * 8, b + i * (16 * 128 / 16), tc_idesc_bf16(kTile, D, true), accumulate || i > 0);
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b_smem, uint32_t b_chunk, int steps, bool accumulate) {
+  const uint64_t b = tc_desc_sw128(b_smem, b_chunk);
+#pragma unroll
+  for (int i = 0; i < kHalf / 16; ++i)
+    if (i < steps) tc_mma_ts(d, a + (i >> 1) * 32 + (i & 1) * 8, b + i * (16 * 128 / 16), tc_idesc_bf16(kTile, D, true), accumulate || i > 0);
 }
 
-// A thread's row of an fp32 accumulator, scaled: bf16 to dst, or fp32 to part (either may be null)
-template <int D>
+// N elements of a thread's row of an fp32 accumulator, scaled: bf16 to dst, or fp32 to part (either may be null)
+template <int N>
 __device__ __forceinline__ void store_row(uint32_t acc, bool has, float scale, bool live, __nv_bfloat16* dst, float* part) {
-#pragma unroll 1
-  for (int i = 0; i < D / 32; ++i) {
-    uint32_t o[32];
+#pragma unroll
+  for (int i = 0; i < N / 16; ++i) {
+    uint32_t o[16];
     __syncwarp();
     if (has) {
-      tc_ld32(acc + i * 32, o);
+      tc_ld16(acc + i * 16, o);
       tc_wait_ld();
     } else {
 #pragma unroll
-      for (int e = 0; e < 32; ++e) o[e] = 0u;
+      for (int e = 0; e < 16; ++e) o[e] = 0u;
     }
     if (!live) continue;
     if (part) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        reinterpret_cast<float4*>(part + i * 32)[e] =
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<float4*>(part + i * 16)[e] =
             make_float4(__uint_as_float(o[4 * e]) * scale, __uint_as_float(o[4 * e + 1]) * scale,
                         __uint_as_float(o[4 * e + 2]) * scale, __uint_as_float(o[4 * e + 3]) * scale);
     } else if (dst) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2; ++e) {
         float f[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[8 * e + x]) * scale;
-        *reinterpret_cast<uint4*>(dst + i * 32 + e * 8) = pack8(f);
+        *reinterpret_cast<uint4*>(dst + i * 16 + e * 8) = pack8(f);
       }
     }
   }
 }
 
-__device__ __forceinline__ float4 lds4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
+// two pairs of floats from shared memory
+__device__ __forceinline__ void lds_pairs(uint32_t addr, f2& a, f2& b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(addr));
 }
+__device__ __forceinline__ f2 pair_of(const uint32_t (&v)[32], int e) { return f2_make(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])); }
+// Pair e of a run of exponentials: some on either unit, so that neither waits for the other.
+__device__ __forceinline__ f2 exp2_mixed(f2 x, int e) { return (e & 3) < kPoly ? exp2_poly(x) : exp2_pair(x); }
 
 // ------------------------------------------------------------------------------------------------ keys: dK, dV
 // grid (key tiles * splits, kv_heads, batch)
@@ -197,14 +208,14 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                           const __grid_constant__ BwdParams p) {
   using C = BwdCfg<D>;
-  constexpr uint32_t kBytes = tile_bytes<D>();
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ volatile int abort_flag;
-  __shared__ uint32_t tmem_slot;
-  const Layout<D> m{(smem_u32(smem_raw) + 1023u) & ~1023u};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr uint32_t kChunk = kHalf * 128;     // bytes of 64 rows of a 64-column chunk
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const Layout<D> m{smem_u32(smem)};
+  volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (m.bar(10) - m.base));
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (m.bar(11) - m.base));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   setup<D>(m, &abort_flag, &tmem_slot, warp);
-  const uint32_t tmem = tmem_slot;
+  constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
   const int split = blockIdx.x % p.splits, jt = blockIdx.x / p.splits, hk = blockIdx.y, b = blockIdx.z;
@@ -213,164 +224,145 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const int first = z.causal ? min(q_tiles, max(0, k0 - off) / kTile) : 0;     // the first query tile with a row that sees a key here
   const int per_head = k0 < n ? q_tiles - first : 0;
   const int begin = split * p.per_split, count = max(0, min(z.group * per_head, begin + p.per_split) - begin);
-  // pass i of this CTA: query tile `tile(i)` of head `head(i)`
+  // pass i of this CTA: query tile `tile(i)` of head `head(i)`; its halves are 2 i and 2 i + 1
   auto head = [&](int i) { return hk * z.group + (begin + i) / per_head; };
   auto tile = [&](int i) { return first + (begin + i) % per_head; };
 
-  if (warp == 9) {
-    // ------------------------------------------------------------ TMA producer: Q0 (with lse2, delta), dO0, Q1, ...
+  if (warp == kTmaWarp) {
+    // ------------------------------------------------------------ TMA producer: a half of q with lse2 and delta, that of dout, ...
     if (lane == 0 && count > 0) {
-      mbar_expect_tx(m.bar(kFixedFull), 2 * kBytes);
-      load_tile<D>(m.fixed(0), &map_k, m.bar(kFixedFull), k0, hk, b);
-      load_tile<D>(m.fixed(1), &map_v, m.bar(kFixedFull), k0, hk, b);
+      mbar_expect_tx(m.bar(kFixedFull), 2 * C::kBytes);
+      load_rows<D, kTile>(m.fixed(0), &map_k, m.bar(kFixedFull), k0, hk, b);
+      load_rows<D, kTile>(m.fixed(1), &map_v, m.bar(kFixedFull), k0, hk, b);
       for (int i = 0; i < 2 * count; ++i) {
-        const int s = i % C::kStages, h = head(i >> 1), q0 = tile(i >> 1) * kTile;
-        if (!mbar_wait(m.empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
-        if (i & 1) {
-          mbar_expect_tx(m.full(s), kBytes);
-          load_tile<D>(m.stage(s), &map_do, m.full(s), q0, h, b);
-        } else {
-          mbar_expect_tx(m.full(s), kBytes + C::kRowBytes);
-          load_tile<D>(m.stage(s), &map_q, m.full(s), q0, h, b);
-          const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + q0;
-          bulk_load(m.row_data(s), p.lse2 + at, kTile * 4, m.full(s));
-          bulk_load(m.row_data(s) + kTile * 4, p.delta + at, kTile * 4, m.full(s));
-        }
+        const int s = i % C::kSlots, h = head(i >> 1), q0 = tile(i >> 1) * kTile + (i & 1) * kHalf;
+        const uint32_t phase = ((i / C::kSlots) & 1) ^ 1;
+        if (!mbar_wait(m.empty(s), phase, &abort_flag)) break;
+        mbar_expect_tx(m.full(s), C::kHalfBytes + C::kRowBytes);
+        load_rows<D, kHalf>(m.q(s), &map_q, m.full(s), q0, h, b);
+        const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + q0;
+        bulk_load(m.row_data(s), p.lse2 + at, kHalf * 4, m.full(s));
+        bulk_load(m.row_data(s) + kHalf * 4, p.delta + at, kHalf * 4, m.full(s));
+        if (!mbar_wait(m.empty2(s), phase, &abort_flag)) break;
+        mbar_expect_tx(m.full2(s), C::kHalfBytes);
+        load_rows<D, kHalf>(m.g(s), &map_do, m.full2(s), q0, h, b);
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
     // share with others their rows are cleared, so that whatever q and dout hold there meets a probability of 0 as 0.
-    auto wait_stage = [&](int i) {
-      if (!warp_wait(m.full(i % C::kStages), (i / C::kStages) & 1, &abort_flag)) return false;
-      if (z.causal && tile(i >> 1) * kTile < -off) zero_rows<D>(m.stage(i % C::kStages), 0, -off - tile(i >> 1) * kTile);
+    auto arrived = [&](int i, bool grad) {
+      const int s = i % C::kSlots;
+      if (!warp_wait(grad ? m.full2(s) : m.full(s), (i / C::kSlots) & 1, &abort_flag)) return false;
+      const int blind = -off - tile(i >> 1) * kTile - (i & 1) * kHalf;
+      if (z.causal && blind > 0) zero_rows<D>(grad ? m.g(s) : m.q(s), kChunk, 0, min(kHalf, blind));
+      tc_fence_after();
       return true;
     };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && wait_stage(0);
-    if (ok) {
+    auto scores = [&](int i) {             // S^T of half i
+      if (!arrived(i, false)) return false;
+      product_ss<D, kHalf>(tmem + C::kS + (i & 1) * kHalf, m.fixed(0), m.q(i % C::kSlots), kChunk);
+      tc_commit_warp(m.bar(kSFull + (i & 1)));
+      return true;
+    };
+    auto gradients = [&](int i) {          // dP^T of half i
+      if (!arrived(i, true)) return false;
+      product_ss<D, kHalf>(tmem + C::kDp + (i & 1) * kHalf, m.fixed(1), m.g(i % C::kSlots), kChunk);
+      tc_commit_warp(m.bar(kDpFull + (i & 1)));
+      return true;
+    };
+    auto add_dv = [&](int i) {             // half i's probabilities are ready: dV += P^T dO, then the scores of the half after next
+      if (!warp_wait(m.bar(kPReady + (i & 1)), (i >> 1) & 1, &abort_flag)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        product_ss<D>(tmem + C::kS, m.fixed(0), m.stage(0));
-        tc_commit(m.bar(kSFull));
-      }
-      ok = wait_stage(1);
+      product_ts<D>(tmem + C::kAcc0, tmem + C::kS + (i & 1) * kHalf, m.g(i % C::kSlots), kChunk, kHalf / 16, i > 0);
+      tc_commit_warp(m.empty2(i % C::kSlots));
+      return i + 2 >= 2 * count || scores(i + 2);
+    };
+    auto add_dk = [&](int i) {             // half i's dS is ready: dK += dS^T Q, then dP of the half after next
+      if (!warp_wait(m.bar(kDsReady + (i & 1)), (i >> 1) & 1, &abort_flag)) return false;
       tc_fence_after();
-      if (ok && lane == 0) {
-        product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage(1));
-        tc_commit(m.bar(kDpFull));
-      }
-      __syncwarp();
-    }
-    for (int i = 0; i < count && ok; ++i) {
-      const int qs = 2 * i % C::kStages, gs = (2 * i + 1) % C::kStages;
-      const bool more = i + 1 < count;
-      ok = warp_wait(m.bar(kPReady), i & 1, &abort_flag) && (!more || wait_stage(2 * i + 2));
-      if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) {
-        product_ts<D>(tmem + C::kAcc0, tmem + C::kS, m.stage(gs), kTile / 16, i > 0);
-        tc_commit(m.empty(gs));
-        if (more) {
-          product_ss<D>(tmem + C::kS, m.fixed(0), m.stage((2 * i + 2) % C::kStages));
-          tc_commit(m.bar(kSFull));
-        }
-      }
-      __syncwarp();
-      ok = warp_wait(m.bar(kDsReady), i & 1, &abort_flag) && (!more || wait_stage(2 * i + 3));
-      if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) {
-        product_ts<D>(tmem + C::kAcc1, tmem + C::kDp, m.stage(qs), kTile / 16, i > 0);
-        if (more) {
-          tc_commit(m.empty(qs));
-          product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage((2 * i + 3) % C::kStages));
-          tc_commit(m.bar(kDpFull));
-        } else {
-          tc_commit(m.bar(kDone));
-        }
-      }
-      __syncwarp();
-    }
+      product_ts<D>(tmem + C::kAcc1, tmem + C::kDp + (i & 1) * kHalf, m.q(i % C::kSlots), kChunk, kHalf / 16, i > 0);
+      tc_commit_warp(m.empty(i % C::kSlots));
+      return i + 2 >= 2 * count || gradients(i + 2);
+    };
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0) && scores(1) && gradients(1);
+    // half a turn apart: P of one half gets ready with dS of the other
+    for (int i = 0; i < 2 * count && ok; ++i) ok = add_dv(i) && (i == 0 || add_dk(i - 1));
+    if (ok && add_dk(2 * count - 1)) tc_commit_warp(m.bar(kDone));
   } else {
-    // ------------------------------------------------------------ probabilities: thread = key, warpgroup w has 64 queries
-    const int w = warp >> 2, row = k0 + (threadIdx.x & 127);
+    // ------------------------------------------------------------ probabilities: thread = key; half g, 32 queries of it
+    const int g = warp >> 3, w = (warp >> 2) & 1, row = k0 + (threadIdx.x & 127);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + C::kS + w * 64, dp_at = tmem + lanes + C::kDp + w * 64;
+    const uint32_t s_at = tmem + lanes + C::kS + g * kHalf + w * 32, dp_at = tmem + lanes + C::kDp + g * kHalf + w * 32;
     const bool row_ok = row < n;
     bool ok = true;
-    const f2 c2 = f2_dup(p.c), minus = f2_dup(-1.f);
+    const f2 c2 = f2_dup(p.c);
     for (int i = 0; i < count; ++i) {
-      const int qs = 2 * i % C::kStages;
-      const int q0 = tile(i) * kTile + w * 64;
-      const uint32_t rows = m.row_data(qs) + w * 256;
-      ok = warp_wait(m.full(qs), (2 * i / C::kStages) & 1, &abort_flag) && warp_wait(m.bar(kSFull), i & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[2][32];
-      tc_ld32(s_at, s[0]);
-      tc_ld32(s_at + 32, s[1]);
-      tc_wait_ld();
-      // queries of this tile before `from` do not see this key
-      const int from = !row_ok ? 64 : (z.causal ? row - off - q0 : 0);
+      const int slot = (2 * i + g) % C::kSlots;
+      const uint32_t rows = m.row_data(slot) + w * 128;
+      // queries of these 32 before `from` do not see this key
+      int from = row_ok ? 0 : 32;
+      if (z.causal && row_ok) from = row - off - tile(i) * kTile - g * kHalf - w * 32;
       const bool edge = __any_sync(0xffffffffu, from > 0);
-      f2 pr[32];
-      uint32_t word[32];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float4 l = lds4(rows + e * 16);
-        const uint32_t* x = &s[e >> 3][(e & 7) * 4];
-        const f2 a = f2_fma(f2_make(__uint_as_float(x[0]), __uint_as_float(x[1])), c2, f2_mul(f2_make(l.x, l.y), minus));
-        const f2 d = f2_fma(f2_make(__uint_as_float(x[2]), __uint_as_float(x[3])), c2, f2_mul(f2_make(l.z, l.w), minus));
-        float y0 = exp2_approx(f2_lo(a)), y1 = exp2_approx(f2_hi(a)), y2 = exp2_approx(f2_lo(d)), y3 = exp2_approx(f2_hi(d));
-        if (edge) {
-          y0 = 4 * e >= from ? y0 : 0.f;
-          y1 = 4 * e + 1 >= from ? y1 : 0.f;
-          y2 = 4 * e + 2 >= from ? y2 : 0.f;
-          y3 = 4 * e + 3 >= from ? y3 : 0.f;
-        }
-        pr[2 * e] = f2_make(y0, y1);
-        pr[2 * e + 1] = f2_make(y2, y3);
-        word[2 * e] = bf16_of_f2(pr[2 * e]);
-        word[2 * e + 1] = bf16_of_f2(pr[2 * e + 1]);
-      }
-      tc_st32(s_at, word);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kPReady));
-
-      ok = warp_wait(m.bar(kDpFull), i & 1, &abort_flag);
+      ok = warp_wait(m.full(slot), ((2 * i + g) / C::kSlots) & 1, &abort_flag) && warp_wait(m.bar(kSFull + g), i & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      tc_ld32(dp_at, s[0]);
-      tc_ld32(dp_at + 32, s[1]);
+      uint32_t s[32], word[16];
+      tc_ld32(s_at, s);
       tc_wait_ld();
+      f2 pr[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float4 l = lds4(rows + kTile * 4 + e * 16);
-        const uint32_t* x = &s[e >> 3][(e & 7) * 4];
-        f2 a = f2_mul(pr[2 * e], f2_fma(f2_make(l.x, l.y), minus, f2_make(__uint_as_float(x[0]), __uint_as_float(x[1]))));
-        f2 d = f2_mul(pr[2 * e + 1], f2_fma(f2_make(l.z, l.w), minus, f2_make(__uint_as_float(x[2]), __uint_as_float(x[3]))));
-        if (!row_ok) a = d = 0ull;        // what lies behind the sample's keys may be NaN
-        word[2 * e] = bf16_of_f2(a);
-        word[2 * e + 1] = bf16_of_f2(d);
+      for (int e = 0; e < 16; e += 2) {
+        f2 l0, l1;
+        lds_pairs(rows + e * 8, l0, l1);
+        pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, l0), e);
+        pr[e + 1] = exp2_mixed(f2_fma(pair_of(s, e + 1), c2, l1), e + 1);
       }
-      tc_st32(dp_at, word);
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pr[e] = f2_make(2 * e >= from ? f2_lo(pr[e]) : 0.f, 2 * e + 1 >= from ? f2_hi(pr[e]) : 0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) word[e] = bf16_of_f2(pr[e]);
+      tc_st16(s_at, word);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kDsReady));
+      if (lane == 0) mbar_arrive(m.bar(kPReady + g));
+
+      ok = warp_wait(m.bar(kDpFull + g), i & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      tc_ld32(dp_at, s);
+      tc_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        f2 d0, d1;
+        lds_pairs(rows + kHalf * 4 + e * 8, d0, d1);
+        word[e] = bf16_of_f2(f2_mul(pr[e], f2_add(pair_of(s, e), d0)));
+        word[e + 1] = bf16_of_f2(f2_mul(pr[e + 1], f2_add(pair_of(s, e + 1), d1)));
+      }
+      if (!row_ok) {                     // what lies behind the sample's keys may be NaN
+#pragma unroll
+        for (int e = 0; e < 16; ++e) word[e] = 0u;
+      }
+      tc_st16(dp_at, word);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(m.bar(kDsReady + g));
     }
     if (ok && count > 0) {
       ok = warp_wait(m.bar(kDone), 0, &abort_flag);
       tc_fence_after();
     }
-    const int64_t at = ((static_cast<int64_t>(b) * z.lk + row) * z.kv_heads + hk) * D;
-    __nv_bfloat16* dst = w == 0 ? p.dv : p.dk;
-    float* part = w == 0 ? p.part0 : p.part1;
-    store_row<D>(tmem + lanes + (w == 0 ? C::kAcc0 : C::kAcc1), count > 0, w == 0 ? 1.f : p.scale, ok && row < z.lk,
-                 dst ? dst + at : nullptr, part ? part + split * p.elements + at : nullptr);
+    // the warpgroups of half 0: the two halves of dV; of half 1: of dK
+    const int64_t at = ((static_cast<int64_t>(b) * z.lk + row) * z.kv_heads + hk) * D + w * (D / 2);
+    __nv_bfloat16* dst = g == 0 ? p.dv : p.dk;
+    float* part = g == 0 ? p.part0 : p.part1;
+    store_row<D / 2>(tmem + lanes + (g == 0 ? C::kAcc0 : C::kAcc1) + w * (D / 2), count > 0, g == 0 ? 1.f : p.scale, ok && row < z.lk,
+                     dst ? dst + at : nullptr, part ? part + split * p.elements + at : nullptr);
   }
   teardown(&abort_flag, p.status, tmem, warp);
 }
@@ -384,15 +376,15 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
                              const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                              const __grid_constant__ BwdParams p) {
   using C = BwdCfg<D>;
-  constexpr uint32_t kBytes = tile_bytes<D>();
-  constexpr uint32_t kS1 = C::kAcc1;       // second buffer of the scores: 256 + D .. 384 + D
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ volatile int abort_flag;
-  __shared__ uint32_t tmem_slot;
-  const Layout<D> m{(smem_u32(smem_raw) + 1023u) & ~1023u};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr uint32_t kS1 = C::kAcc1;       // second buffer of the scores
+  constexpr uint32_t kChunk = kTile * 128;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const Layout<D> m{smem_u32(smem)};
+  volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (m.bar(10) - m.base));
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (m.bar(11) - m.base));
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   setup<D>(m, &abort_flag, &tmem_slot, warp);
-  const uint32_t tmem = tmem_slot;
+  constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
   const int split = blockIdx.x % p.splits, qt = blockIdx.x / p.splits, h = blockIdx.y, b = blockIdx.z;
@@ -400,125 +392,107 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
   const int lim_tile = key_limit(z, n, min(z.lq, q0 + kTile) - 1);
   const int j0 = split * p.per_split, count = max(0, min((lim_tile + kTile - 1) / kTile, j0 + p.per_split) - j0);
 
-  if (warp == 9) {
+  if (warp == kTmaWarp) {
     // ------------------------------------------------------------ TMA producer: K0, V0, K1, V1, ...
     if (lane == 0 && count > 0) {
-      mbar_expect_tx(m.bar(kFixedFull), 2 * kBytes);
-      load_tile<D>(m.fixed(0), &map_q, m.bar(kFixedFull), q0, h, b);
-      load_tile<D>(m.fixed(1), &map_do, m.bar(kFixedFull), q0, h, b);
+      mbar_expect_tx(m.bar(kFixedFull), 2 * C::kBytes);
+      load_rows<D, kTile>(m.fixed(0), &map_q, m.bar(kFixedFull), q0, h, b);
+      load_rows<D, kTile>(m.fixed(1), &map_do, m.bar(kFixedFull), q0, h, b);
       for (int i = 0; i < 2 * count; ++i) {
         const int s = i % C::kStages;
         if (!mbar_wait(m.empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
-        mbar_expect_tx(m.full(s), kBytes);
-        load_tile<D>(m.stage(s), (i & 1) ? &map_v : &map_k, m.full(s), (j0 + (i >> 1)) * kTile, hk, b);
+        mbar_expect_tx(m.full(s), C::kBytes);
+        load_rows<D, kTile>(m.stage(s), (i & 1) ? &map_v : &map_k, m.full(s), (j0 + (i >> 1)) * kTile, hk, b);
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     auto wait_stage = [&](int i) { return warp_wait(m.full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
-    auto steps_of = [&](int j) { return (min(kTile, n - (j0 + j) * kTile) + 15) / 16; };
+    auto keys_in = [&](int j) { return min(kTile, n - (j0 + j) * kTile); };
     auto scores = [&](int j) {             // S(j) = Q K_j^T; the keys' rows behind the sample's length are cleared for dS K
       if (!wait_stage(2 * j)) return false;
-      const int keys = min(kTile, n - (j0 + j) * kTile);
-      if (keys & 15) zero_rows<D>(m.stage(2 * j % C::kStages), keys, steps_of(j) * 16);
+      const int keys = keys_in(j);
+      if (keys & 15) zero_rows<D>(m.stage(2 * j % C::kStages), kChunk, keys, (keys + 15) & ~15);
       tc_fence_after();
-      if (lane == 0) {
-        product_ss<D>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(2 * j % C::kStages));
-        tc_commit(m.bar(kSFull + (j & 1)));
-      }
-      __syncwarp();
+      product_ss<D, kTile>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(2 * j % C::kStages), kChunk);
+      tc_commit_warp(m.bar(kSFull + (j & 1)));
       return true;
     };
-    auto gradients = [&](int j) {          // dP(j) = dO V_j^T
+    auto gradients = [&](int j, int g) {   // half g of dP(j) = dO V_j^T
+      const int s = (2 * j + 1) % C::kStages;
       if (!wait_stage(2 * j + 1)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage((2 * j + 1) % C::kStages));
-        tc_commit(m.bar(kDpFull));
-        tc_commit(m.empty((2 * j + 1) % C::kStages));
-      }
-      __syncwarp();
+      product_ss<D, kHalf>(tmem + C::kDp + g * kHalf, m.fixed(1), m.stage(s) + g * (kHalf * 128), kChunk);
+      tc_commit_warp(m.bar(kDpFull + g));
+      if (g == 1) tc_commit_warp(m.empty(s));
       return true;
     };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0) && (count == 1 || scores(1));
-    for (int j = 0; j < count && ok; ++j) {
-      ok = warp_wait(m.bar(kDsReady), j & 1, &abort_flag);
-      if (!ok) break;
+    auto add_dq = [&](int j, int g) {      // half g of dS(j) is ready: dQ += dS K
+      const int s = 2 * j % C::kStages;
+      if (!warp_wait(m.bar(kDsReady + g), j & 1, &abort_flag)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        product_ts<D>(tmem + C::kAcc0, tmem + C::kDp, m.stage(2 * j % C::kStages), steps_of(j), j > 0);
-        tc_commit(j + 1 < count ? m.empty(2 * j % C::kStages) : m.bar(kDone));
-      }
-      __syncwarp();
-      if (j + 1 < count) ok = gradients(j + 1);
-      if (ok && j + 2 < count) ok = scores(j + 2);
+      const int steps = (min(kHalf, keys_in(j) - g * kHalf) + 15) / 16;
+      product_ts<D>(tmem + C::kAcc0, tmem + C::kDp + g * kHalf, m.stage(s) + g * (kHalf * 128), kChunk, steps, j > 0 || g > 0);
+      if (g == 1) tc_commit_warp(m.empty(s));
+      return true;
+    };
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0, 0) && gradients(0, 1) &&
+              (count == 1 || scores(1));
+    for (int j = 0; j < count && ok; ++j) {
+      const bool more = j + 1 < count;
+      ok = add_dq(j, 0) && (!more || gradients(j + 1, 0)) && add_dq(j, 1) && (!more || gradients(j + 1, 1)) &&
+           (j + 2 >= count || scores(j + 2));
     }
+    if (ok && count > 0) tc_commit_warp(m.bar(kDone));
   } else {
-    // ------------------------------------------------------------ probabilities: thread = query, warpgroup w has 64 keys
-    const int w = warp >> 2, row = q0 + (threadIdx.x & 127);
+    // ------------------------------------------------------------ probabilities: thread = query; half g, 32 keys of it
+    const int g = warp >> 3, w = (warp >> 2) & 1, row = q0 + (threadIdx.x & 127), col = g * kHalf + w * 32;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t dp_at = tmem + lanes + C::kDp + w * 64;
+    const uint32_t dp_at = tmem + lanes + C::kDp + col;
     const int lim = key_limit(z, n, row);
     const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
     const int64_t r = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + row;
-    const f2 c2 = f2_dup(p.c), lse = f2_dup(-p.lse2[r]), delta = f2_dup(-p.delta[r]);
+    const f2 c2 = f2_dup(p.c), lse = f2_dup(p.lse2[r]), delta = f2_dup(p.delta[r]);
     bool ok = true;
     for (int j = 0; j < count; ++j) {
       ok = warp_wait(m.bar(kSFull + (j & 1)), (j >> 1) & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t s_at = tmem + lanes + ((j & 1) ? kS1 : C::kS) + w * 64;
-      uint32_t s[2][32];
-      tc_ld32(s_at, s[0]);
-      tc_ld32(s_at + 32, s[1]);
+      uint32_t s[32], word[16];
+      tc_ld32(tmem + lanes + ((j & 1) ? kS1 : C::kS) + col, s);
       tc_wait_ld();
-      const int k0 = (j0 + j) * kTile + w * 64;
-      const bool edge = k0 + 64 > lim_all;
-      f2 pr[32];
+      f2 pr[16];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const uint32_t* x = &s[e >> 4][(e & 15) * 2];
-        const f2 a = f2_fma(f2_make(__uint_as_float(x[0]), __uint_as_float(x[1])), c2, lse);
-        float y0 = exp2_approx(f2_lo(a)), y1 = exp2_approx(f2_hi(a));
-        if (edge) {
-          y0 = k0 + 2 * e < lim ? y0 : 0.f;
-          y1 = k0 + 2 * e + 1 < lim ? y1 : 0.f;
-        }
-        pr[e] = f2_make(y0, y1);
-      }
-      ok = warp_wait(m.bar(kDpFull), j & 1, &abort_flag);
+      for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, lse), e);
+      ok = warp_wait(m.bar(kDpFull + g), j & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      tc_ld32(dp_at, s[0]);
-      tc_ld32(dp_at + 32, s[1]);
+      tc_ld32(dp_at, s);
       tc_wait_ld();
-      uint32_t word[32];
+      const int from = lim - (j0 + j) * kTile - col;         // keys from here on are not seen
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const uint32_t* x = &s[e >> 4][(e & 15) * 2];
-        const f2 a = f2_mul(pr[e], f2_add(f2_make(__uint_as_float(x[0]), __uint_as_float(x[1])), delta));
-        float y0 = f2_lo(a), y1 = f2_hi(a);
-        if (edge) {                        // what lies behind the sample's keys may be NaN
-          y0 = k0 + 2 * e < lim ? y0 : 0.f;
-          y1 = k0 + 2 * e + 1 < lim ? y1 : 0.f;
-        }
-        word[e] = bf16_of_f2(f2_make(y0, y1));
+      for (int e = 0; e < 16; ++e) pr[e] = f2_mul(pr[e], f2_add(pair_of(s, e), delta));
+      if ((j0 + j) * kTile + col + 32 > lim_all) {           // what lies behind the sample's keys may be NaN
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pr[e] = f2_make(2 * e < from ? f2_lo(pr[e]) : 0.f, 2 * e + 1 < from ? f2_hi(pr[e]) : 0.f);
       }
-      tc_st32(dp_at, word);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) word[e] = bf16_of_f2(pr[e]);
+      tc_st16(dp_at, word);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kDsReady));
+      if (lane == 0) mbar_arrive(m.bar(kDsReady + g));
     }
     if (ok && count > 0) {
       ok = warp_wait(m.bar(kDone), 0, &abort_flag);
       tc_fence_after();
     }
-    if (w == 0) {
-      const int64_t dense = ((static_cast<int64_t>(b) * z.heads + h) * z.lq + row) * D;
-      store_row<D>(tmem + lanes + C::kAcc0, count > 0, p.scale, ok && row < z.lq,
-                   p.dq + b * p.sdq.b + row * p.sdq.l + h * p.sdq.h, p.part0 ? p.part0 + split * p.elements + dense : nullptr);
-    }
+    const int quarter = warp >> 2;
+    const int64_t dense = ((static_cast<int64_t>(b) * z.heads + h) * z.lq + row) * D + quarter * (D / 4);
+    store_row<D / 4>(tmem + lanes + C::kAcc0 + quarter * (D / 4), count > 0, p.scale, ok && row < z.lq,
+                     p.dq + b * p.sdq.b + row * p.sdq.l + h * p.sdq.h + quarter * (D / 4),
+                     p.part0 ? p.part0 + split * p.elements + dense : nullptr);
   }
   teardown(&abort_flag, p.status, tmem, warp);
 }
@@ -610,7 +584,7 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
     p.part0 = p.splits > 1 ? part : nullptr;
     p.part1 = p.splits > 1 ? part + p.splits * p.elements : nullptr;
     const dim3 grid(static_cast<unsigned>(ceil_div(s.lk, kTile) * p.splits), static_cast<unsigned>(s.kv_heads), static_cast<unsigned>(s.batch));
-    launch_after(attention_bwd_keys_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
+    launch_after(attention_bwd_keys_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[4], maps[5], maps[2], maps[3], p);
     ANIMA_CHECK_LAUNCH(who);
     if (p.splits > 1) {
       if (p.dv)
@@ -699,9 +673,11 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
   rows.heads = p.z.heads;
   rows.rows = s.batch * plan.lq_pad * s.heads;
   const void* stand_in = no_q ? k : q;
-  CUtensorMap maps[4];
+  CUtensorMap maps[6];                   // whole tiles of q, dout, k, v; half tiles of q and dout
   ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, stand_in) &&
                     attn::encode_heads(&maps[1], dout, sdo, s.batch, s.lq, s.heads, s.d, stand_in) &&
+                    attn::encode_heads(&maps[4], q, sq, s.batch, s.lq, s.heads, s.d, stand_in, attn::kHalf) &&
+                    attn::encode_heads(&maps[5], dout, sdo, s.batch, s.lq, s.heads, s.d, stand_in, attn::kHalf) &&
                     attn::encode_heads(&maps[2], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in) &&
                     attn::encode_heads(&maps[3], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in),
                 ANIMA_E_CUDA, "%s: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand)", who);

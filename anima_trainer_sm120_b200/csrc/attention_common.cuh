@@ -30,10 +30,34 @@ __device__ __forceinline__ int keys_of(const Sizes& z, int b) { return z.lengths
 // keys that query i of a sample with n keys sees are 0 .. limit - 1
 __device__ __forceinline__ int key_limit(const Sizes& z, int n, int i) { return z.causal ? max(0, min(n, i + z.lk - z.lq + 1)) : n; }
 
-// 2^x
+// 2^x on the special-function unit, of which an SM finishes 16 a cycle
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^x on the multiply-add pipes, two values at once: x = n + f, n the nearest integer, |f| <= 1/2; 2^f by a polynomial of degree
+// 4 with value 1 at 0, fitted to the least relative error (Lawson's weighted least squares; 2.9e-6 in fp32 arithmetic,
+// which the rounding of the result to bf16 exceeds a thousand times). Adding 1.5 2^23 + 127 rounds to n and leaves n + 127 in
+// the low bits, the exponent of 2^n. Below -126.5 that is 0 and so is the result; NaN stays NaN. x at most 127.
+__device__ __forceinline__ f2 exp2_poly(f2 x) {
+  float lo, hi;
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(lo) : "f"(f2_lo(x)));     // -127
+  asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(hi) : "f"(f2_hi(x)));
+  x = f2_make(lo, hi);
+  const f2 t = f2_add(x, f2_dup(12583039.f));
+  const f2 f = f2_fma(f2_add(t, f2_dup(-12583039.f)), f2_dup(-1.f), x);
+  f2 p = f2_fma(f, f2_dup(0.009582852944731712f), f2_dup(0.055906426161527634f));
+  p = f2_fma(p, f, f2_dup(0.24024099111557007f));
+  p = f2_fma(p, f, f2_dup(0.6931241750717163f));
+  p = f2_fma(p, f, f2_dup(1.f));
+  const uint32_t a = static_cast<uint32_t>(t), b = static_cast<uint32_t>(t >> 32);
+  return f2_mul(p, f2_make(__uint_as_float(a << 23), __uint_as_float(b << 23)));
+}
+__device__ __forceinline__ f2 exp2_pair(f2 x) { return f2_make(exp2_approx(f2_lo(x)), exp2_approx(f2_hi(x))); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 __device__ __forceinline__ float log2_approx(float x) {
@@ -44,6 +68,7 @@ __device__ __forceinline__ float log2_approx(float x) {
 
 // A wait of a whole warp with one answer for all its lanes.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
@@ -52,25 +77,25 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-// A tile of 128 tokens of one head: D / 64 chunks of 128 rows x 128 bytes (swizzled), one behind the other. Tokens behind the
-// last one arrive as zeros.
-template <int D>
-__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int token, int head, int b) {
+// ROWS tokens of one head: D / 64 chunks of ROWS x 128 bytes (swizzled), one behind the other. Tokens behind the last one arrive
+// as zeros.
+template <int D, int ROWS>
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int token, int head, int b) {
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) tma_load_4d(dst + c * (kTile * 128), map, bar, c * 64, token, head, b);
+  for (int c = 0; c < D / 64; ++c) tma_load_4d(dst + c * (ROWS * 128), map, bar, c * 64, token, head, b);
 }
 template <int D>
 constexpr uint32_t tile_bytes() { return kTile * D * 2; }
 
-// Rows first .. last - 1 of a tile in shared memory become zero (a whole warp): what TMA brought from behind a sample's
-// length may be NaN, which a product with a probability of 0 would spread.
+// Rows first .. last - 1 of a tile in shared memory (chunks `chunk` bytes apart) become zero (a whole warp): what TMA brought from
+// behind a sample's length may be NaN, which a product with a probability of 0 would spread.
 template <int D>
-__device__ __forceinline__ void zero_rows(uint32_t tile, int first, int last) {
+__device__ __forceinline__ void zero_rows(uint32_t tile, uint32_t chunk, int first, int last) {
   const int lane = threadIdx.x & 31;
   for (int i = first * 8 + lane; i < last * 8; i += 32) {
 #pragma unroll
     for (int c = 0; c < D / 64; ++c)
-      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * (kTile * 128) + i * 16), "r"(0) : "memory");
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + c * chunk + i * 16), "r"(0) : "memory");
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
@@ -130,10 +155,10 @@ inline bool bind_context() {
   return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
-// Tensor map of a (batch, token, head, D) bf16 tensor, boxes of 128 tokens x 64 elements. A tensor without elements gets the
+// Tensor map of a (batch, token, head, D) bf16 tensor, boxes of `rows` tokens x 64 elements. A tensor without elements gets the
 // map of one that is never read (`stand_in`: any valid address).
 inline bool encode_heads(CUtensorMap* map, const void* p, const Strided& s, int64_t batch, int64_t len, int64_t heads, int64_t d,
-                         const void* stand_in) {
+                         const void* stand_in, uint32_t rows = kTile) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   const bool none = batch * len == 0;
@@ -141,7 +166,7 @@ inline bool encode_heads(CUtensorMap* map, const void* p, const Strided& s, int6
   // the stride of a dimension of one element is not used; any valid one will do
   auto bytes = [&](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 && !none ? stride * 2 : 2 * d); };
   const cuuint64_t strides[3] = {bytes(len, s.l), bytes(heads, s.h), bytes(batch, s.b)};
-  const cuuint32_t box[4] = {64, kTile, 1, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, rows, 1, 1}, step[4] = {1, 1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(none ? stand_in : p), dims, strides, box, step,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

@@ -1,19 +1,20 @@
 // Attention, forward (formulas: attention_common.cuh): one pass over the keys with each row's running maximum and sum.
 //
-// A CTA owns two tiles of 128 queries of one head and walks the keys in tiles of 128. Per tile and key tile
+// A CTA owns two tiles of 128 queries of one head and walks the keys, 64 at a time. Per query tile and step
 //   S = Q K^T     tcgen05, both operands in shared memory, fp32 scores in tensor memory (lane = query, column = key);
-//   softmax       one warpgroup a query tile, one thread a row: 128 scores into registers, row maximum without shuffles,
+//   softmax       one warpgroup a query tile, one thread a row: 64 scores into registers, row maximum without shuffles,
 //                 p = 2^(s scale log2 e - m), rounded to bf16 for the second product (the sum takes the unrounded values), written
 //                 over the scores;
 //   O += P V      tcgen05 with P read from tensor memory, V as it lies (keys along rows: the MN-major form), fp32.
-// The two tiles alternate: while one is in its softmax, the tensor cores work for the other. Warp 8 issues the products, warp
-// 9 feeds K and V tiles through a ring of TMA boxes.
+// The scores of a query tile have two buffers: S of the step after next is issued behind O += P V, which frees its buffer, so
+// a warpgroup finds its next scores ready and the special-function unit, shared by both, never waits for the tensor cores.
+// One warp issues the products, one feeds tiles of 128 keys of K and V through a ring of TMA boxes.
 // The running maximum of a row is only raised once a score exceeds it by 2^8: until then p is at most 256, which costs neither
 // bf16 (relative) nor the fp32 sums anything, and O, which lies in tensor memory, need not be rescaled.
 // Few rows (one token, a short text) leave SMs idle: the keys are then cut into ranges, whose normalised fp32 outputs and
 // log-sums a second kernel joins in order. One query token per sample: the heads that share a key head become the rows of a
 // tile, so that each key is read once.
-// Bound: 4 D flop a (query, key) pair on the tensor cores and one exponential, of which an SM makes 16 a cycle: a tile
+// Bound: 4 D flop a (query, key) pair on the tensor cores and one exponential, of which an SM makes 16 a cycle: a tile pair
 // of D = 128 takes 1024 cycles of either.
 #include "attention_common.cuh"
 
@@ -22,14 +23,17 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 320;            // two softmax warpgroups, one MMA warp, one TMA warp
+constexpr int kStep = 64;                // keys of a step
 constexpr float kMaxSlack = 8.f;         // log2 of how far a score may exceed the maximum in use
+constexpr int kPoly = 0;                 // of four pairs of exponentials, those made on the multiply-add pipes
 
 template <int D>
 struct FwdCfg {
   static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kBars = 2 * kStages + 7;
-  static constexpr int kSmem = (2 + kStages) * static_cast<int>(tile_bytes<D>()) + 1024 + kBars * 8 + 16;
-  // tensor-memory columns
+  static constexpr int kBars = 2 * kStages + 13;
+  static constexpr int kSmem = (2 + kStages) * static_cast<int>(tile_bytes<D>()) + kBars * 8;
+  static_assert(kSmem <= 227 * 1024 - 16, "shared memory");
+  // tensor-memory columns: scores of tile t, buffer x at 128 t + 64 x
   static constexpr uint32_t kS = 0, kO = 256;
 };
 
@@ -53,33 +57,24 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
   using C = FwdCfg<D>;
   constexpr uint32_t kBytes = tile_bytes<D>();
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ volatile int abort_flag;
   __shared__ uint32_t tmem_slot;
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t base = smem_u32(smem);
   auto q_smem = [&](int t) { return base + t * kBytes; };
   auto kv_smem = [&](int s) { return base + (2 + s) * kBytes; };
   const uint32_t bars = base + (2 + C::kStages) * kBytes;
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
   const uint32_t q_full = bars + 8 * (2 * C::kStages);
-  auto s_full = [&](int t) { return q_full + 8 * (1 + t); };
-  auto p_full = [&](int t) { return q_full + 8 * (3 + t); };
-  auto o_done = [&](int t) { return q_full + 8 * (5 + t); };
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto s_full = [&](int t, int x) { return q_full + 8 * (1 + 2 * t + x); };
+  auto p_full = [&](int t, int x) { return q_full + 8 * (5 + 2 * t + x); };
+  auto o_done = [&](int t, int x) { return q_full + 8 * (9 + 2 * t + x); };
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), 1);
-      mbar_init(empty(s), 1);
-    }
-    mbar_init(q_full, 1);
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(s_full(t), 1);
-      mbar_init(p_full(t), 4);
-      mbar_init(o_done(t), 1);
-    }
+    for (int i = 0; i < C::kBars; ++i) mbar_init(bars + 8 * i, i >= 2 * C::kStages + 5 && i < 2 * C::kStages + 9 ? 4 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
@@ -90,22 +85,22 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   __syncthreads();
   tc_fence_after();
   after_previous();
-  const uint32_t tmem = tmem_slot;
+  constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
   const int split = blockIdx.x / p.q_blocks, qb = blockIdx.x - split * p.q_blocks, h = blockIdx.y, b = blockIdx.z;
   const int hk = h / z.group;
   const int q0 = qb * 2 * kTile;
   const int n = keys_of(z, b);
-  // key tiles this CTA walks for each query tile: [j0, j0 + count[t])
-  const int j0 = split * p.tiles_per_split;
+  // this CTA's keys start at k0; query tile t takes count[t] steps
+  const int j0 = split * p.tiles_per_split, k0 = j0 * kTile;
   int count[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int first = q0 + t * kTile;
     const int last = min(z.lq, first + kTile) - 1;
-    const int lim = first < z.lq ? key_limit(z, n, last) : 0;
-    count[t] = max(0, min((lim + kTile - 1) / kTile, j0 + p.tiles_per_split) - j0);
+    const int lim = first < z.lq ? min(key_limit(z, n, last), k0 + p.tiles_per_split * kTile) : 0;
+    count[t] = max(0, lim - k0 + kStep - 1) / kStep;
   }
   const int most = max(count[0], count[1]);
 
@@ -113,69 +108,66 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     // ------------------------------------------------------------ TMA producer: K0, V0, K1, V1, ...
     if (lane == 0 && most > 0) {
       mbar_expect_tx(q_full, kBytes * (count[1] > 0 ? 2 : 1));
-      load_tile<D>(q_smem(0), &map_q, q_full, q0, h, b);
-      if (count[1] > 0) load_tile<D>(q_smem(1), &map_q, q_full, q0 + kTile, h, b);
-      for (int i = 0; i < 2 * most; ++i) {
+      load_rows<D, kTile>(q_smem(0), &map_q, q_full, q0, h, b);
+      if (count[1] > 0) load_rows<D, kTile>(q_smem(1), &map_q, q_full, q0 + kTile, h, b);
+      for (int i = 0; i < 2 * ((most + 1) / 2); ++i) {
         const int s = i % C::kStages;
         if (!mbar_wait(empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
         mbar_expect_tx(full(s), kBytes);
-        load_tile<D>(kv_smem(s), (i & 1) ? &map_v : &map_k, full(s), (j0 + (i >> 1)) * kTile, hk, b);
+        load_rows<D, kTile>(kv_smem(s), (i & 1) ? &map_v : &map_k, full(s), k0 + (i >> 1) * kTile, hk, b);
       }
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------ MMA issuer
-    constexpr uint32_t kIdescS = tc_idesc_bf16(kTile, kTile), kIdescO = tc_idesc_bf16(kTile, D, true);
-    auto scores = [&](int t, int stage) {      // S_t = Q_t K^T
-      const uint64_t a = tc_desc_sw128(q_smem(t)), k = tc_desc_sw128(kv_smem(stage));
+    constexpr uint32_t kIdescS = tc_idesc_bf16(kTile, kStep), kIdescO = tc_idesc_bf16(kTile, D, true);
+    auto k_stage = [&](int u) { return (u >> 1) * 2 % C::kStages; };
+    auto v_stage = [&](int u) { return ((u >> 1) * 2 + 1) % C::kStages; };
+    auto arrived = [&](int i) { return warp_wait(full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
+    auto scores = [&](int t, int u) {          // S of query tile t and step u 
+      const uint64_t a = tc_desc_sw128(q_smem(t)), k = tc_desc_sw128(kv_smem(k_stage(u)) + (u & 1) * (kStep * 128));
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const uint32_t at = (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2;   // 16 bytes a unit
-        tc_mma_ss(tmem + C::kS + t * kTile, a + at, k + at, kIdescS, i > 0);
+        tc_mma_ss(tmem + C::kS + t * kTile + (u & 1) * kStep, a + at, k + at, kIdescS, i > 0);
       }
-      tc_commit(s_full(t));
+      tc_commit_warp(s_full(t, u & 1));
     };
-    bool ok = most > 0 && warp_wait(q_full, 0, &abort_flag) && warp_wait(full(0), 0, &abort_flag);
+    bool ok = most > 0 && warp_wait(q_full, 0, &abort_flag) && arrived(0);
     if (ok) {
       tc_fence_after();
-      if (lane == 0) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (count[t] > 0) scores(t, 0);
-        tc_commit(empty(0));
-      }
-      __syncwarp();
+          if (u < count[t]) scores(t, u);
+      tc_commit_warp(empty(0));
     }
-    for (int j = 0; j < most && ok; ++j) {
-      const int vi = 2 * j + 1, vs = vi % C::kStages, ki = 2 * j + 2, ks = ki % C::kStages;
-      // keys of the tile that exist; the product over the others is left out, up to the next multiple of 16
-      const int keys = min(kTile, n - (j0 + j) * kTile), steps = (keys + 15) / 16;
-      ok = warp_wait(full(vs), (vi / C::kStages) & 1, &abort_flag);
+    for (int u = 0; u < most && ok; ++u) {
+      const int vs = v_stage(u);
+      const bool next = u + 2 < most;
+      // keys of the step that exist; the product over the others is left out, up to the next multiple of 16
+      const int keys = min(kStep, n - k0 - u * kStep), steps = (keys + 15) / 16;
+      if (!(u & 1)) ok = arrived((u >> 1) * 2 + 1) && (!next || arrived((u >> 1) * 2 + 2));
       if (!ok) break;
-      if (keys & 15) zero_rows<D>(kv_smem(vs), keys, steps * 16);
-      const uint64_t v = tc_desc_sw128(kv_smem(vs), kTile * 128);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (j >= count[t]) continue;
-        ok = warp_wait(p_full(t), j & 1, &abort_flag);
+      if (keys & 15) zero_rows<D>(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128, keys, steps * 16);
+      const uint64_t v = tc_desc_sw128(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (u >= count[t]) continue;
+        ok = warp_wait(p_full(t, u & 1), (u >> 1) & 1, &abort_flag);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t o = tmem + C::kO + t * D, pr = tmem + C::kS + t * kTile;
-          for (int i = 0; i < steps; ++i) tc_mma_ts(o, pr + i * 8, v + i * (16 * 128 / 16), kIdescO, j > 0 || i > 0);
-          tc_commit(o_done(t));
-        }
-        __syncwarp();
-        if (j + 1 < count[t]) {
-          ok = warp_wait(full(ks), (ki / C::kStages) & 1, &abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane == 0) scores(t, ks);
-          __syncwarp();
-        }
+        const uint32_t o = tmem + C::kO + t * D, pr = tmem + C::kS + t * kTile + (u & 1) * kStep;
+#pragma unroll
+        for (int i = 0; i < kStep / 16; ++i)
+          if (i < steps) tc_mma_ts(o, pr + i * 8, v + i * (16 * 128 / 16), kIdescO, u > 0 || i > 0);
+        tc_commit_warp(o_done(t, u & 1));
+        if (u + 2 < count[t]) scores(t, u + 2);
       }
-      if (ok && lane == 0) {
-        tc_commit(empty(vs));
-        if (j + 1 < most) tc_commit(empty(ks));
+      if (ok && (u & 1)) {
+        tc_commit_warp(empty(vs));
+        if (next) tc_commit_warp(empty(k_stage(u + 2)));
       }
-      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ softmax: warpgroup t, thread = row
@@ -184,32 +176,32 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + C::kS + t * kTile, o_at = tmem + lanes + C::kO + t * D;
     const int lim = key_limit(z, n, row);
-    // the warp's first row sees the fewest keys: tiles that end before that need no mask
+    // the warp's first row sees the fewest keys: steps that end before that need no mask
     const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
     float m = -INFINITY, l = 0.f, used = 0.f;      // maximum in use (raw scores), sum, m * c (0 while there is none)
     bool ok = true;
-    for (int j = 0; j < count[t]; ++j) {
-      ok = warp_wait(s_full(t), j & 1, &abort_flag);
+    for (int u = 0; u < count[t]; ++u) {
+      const uint32_t at = s_at + (u & 1) * kStep;
+      ok = warp_wait(s_full(t, u & 1), (u >> 1) & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tc_ld32(s_at + i * 32, s[i]);
+      uint32_t s[2][32];
+      tc_ld32(at, s[0]);
+      tc_ld32(at + 32, s[1]);
       tc_wait_ld();
-      const int k0 = (j0 + j) * kTile;
-      if (k0 + kTile > lim_all) {
+      const int key = k0 + u * kStep;
+      if (key + kStep > lim_all) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if (k0 + i * 32 + e >= lim) s[i][e] = 0xff800000u;
+            if (key + i * 32 + e >= lim) s[i][e] = 0xff800000u;
       }
       float mx[4] = {m, m, m, m};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 32; e += 2)
-          mx[i] = fmaxf(mx[i], fmaxf(__uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1])));
+        for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool grow = (top - m) * p.c > kMaxSlack;
       if (__any_sync(0xffffffffu, grow)) {
@@ -219,8 +211,8 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           l *= f;
           used = m * p.c;
         }
-        if (j > 0) {
-          ok = warp_wait(o_done(t), (j - 1) & 1, &abort_flag);
+        if (u > 0) {                       // the product of the step before is the last one under way: S(u) came behind the others
+          ok = warp_wait(o_done(t, (u - 1) & 1), ((u - 1) >> 1) & 1, &abort_flag);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -235,29 +227,30 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
       }
       const f2 c2 = f2_dup(p.c), u2 = f2_dup(-used);
-      f2 sum0 = 0ull, sum1 = 0ull;
+      f2 sum[4] = {0ull, 0ull, 0ull, 0ull}, y[32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const f2 x = f2_fma(f2_make(__uint_as_float(s[i][2 * e]), __uint_as_float(s[i][2 * e + 1])), c2, u2);
-          const f2 y = f2_make(exp2_approx(f2_lo(x)), exp2_approx(f2_hi(x)));
-          if (e & 1) sum1 = f2_add(sum1, y);
-          else sum0 = f2_add(sum0, y);
-          w[e] = bf16_of_f2(y);
+          y[i * 16 + e] = (e & 3) < kPoly ? exp2_poly(x) : exp2_pair(x);
+          w[e] = bf16_of_f2(y[i * 16 + e]);
         }
-        tc_st16(s_at + i * 16, w);
+        tc_st16(at + i * 16, w);
       }
-      l += f2_sum(f2_add(sum0, sum1));
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(t));
+      if (lane == 0) mbar_arrive(p_full(t, u & 1));
+      // the row's sum, behind what the tensor cores wait for
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sum[e & 3] = f2_add(sum[e & 3], y[e]);
+      l += f2_sum(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])));
     }
     // ------------------------------------------------------------ epilogue
     if (ok && count[t] > 0) {
-      ok = warp_wait(o_done(t), (count[t] - 1) & 1, &abort_flag);
+      ok = warp_wait(o_done(t, (count[t] - 1) & 1), ((count[t] - 1) >> 1) & 1, &abort_flag);
       tc_fence_after();
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;        // a row without keys has no sum
