@@ -15,7 +15,8 @@
 // of another.
 // A query tile (keys kernel) or key tile (queries kernel) is taken in two halves of 64, each with tensor memory, barriers and two
 // of the four warpgroups of its own: while one half makes exponentials, the other makes dS, and the tensor cores work on what
-// either has finished. One warp issues all products, in the order in which the halves get ready.
+// either has finished. Two warps issue the products (keys: one S and dV, one dP and dK; queries: one S, one dP and dQ), so that
+// the waits of one overlap the products of the other.
 // Bound: 14 D flop a (query, key) pair on the tensor cores; two exponentials.
 #include "attention_common.cuh"
 
@@ -24,7 +25,7 @@ namespace attn {
 namespace {
 
 constexpr int kWorkers = 16;             // warps that make probabilities: two warpgroups for each half of a tile
-constexpr int kMmaWarp = kWorkers, kTmaWarp = kWorkers + 1, kThreads = (kWorkers + 2) * 32;
+constexpr int kMmaWarp = kWorkers, kTmaWarp = kWorkers + 2, kThreads = (kWorkers + 3) * 32;   // two warps issue products
 constexpr int kHalf = kTile / 2;
 constexpr int kPoly = 0;                 // of four pairs of exponentials, those made on the multiply-add pipes
 
@@ -111,13 +112,18 @@ struct Layout {
 // one barrier each, or one for each half (or score buffer)
 enum { kFixedFull = 0, kDone = 1, kSFull = 2, kDpFull = 4, kPReady = 6, kDsReady = 8 };
 
-template <int D>
+template <int D, bool KEYS>
 __device__ __forceinline__ void setup(const Layout<D>& m, volatile int* abort_flag, uint32_t* tmem_slot, int warp) {
   using C = BwdCfg<D>;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < C::kBars; ++i)
-      if (i < 10 || i >= 12) mbar_init(m.bar(i), i >= kPReady && i < kDsReady + 2 ? kWorkers / 2 : 1);
+    for (int i = 0; i < C::kBars; ++i) {
+      int arrivals = 1;
+      if (i >= kPReady && i < kPReady + 2) arrivals = KEYS ? kWorkers / 2 : kWorkers;      // queries: S(j) has been read
+      if (i >= kDsReady && i < kDsReady + 2) arrivals = kWorkers / 2;
+      if (KEYS && (i == kDone || i >= 12 + 3 * C::kSlots)) arrivals = 2;                   // both MMA warps
+      if (i < 10 || i >= 12) mbar_init(m.bar(i), arrivals);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) tc_alloc(smem_u32(tmem_slot), 512);
@@ -214,7 +220,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (m.bar(10) - m.base));
   uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (m.bar(11) - m.base));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  setup<D>(m, &abort_flag, &tmem_slot, warp);
+  setup<D, true>(m, &abort_flag, &tmem_slot, warp);
   constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
@@ -227,6 +233,11 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   // pass i of this CTA: query tile `tile(i)` of head `head(i)`; its halves are 2 i and 2 i + 1
   auto head = [&](int i) { return hk * z.group + (begin + i) / per_head; };
   auto tile = [&](int i) { return first + (begin + i) % per_head; };
+  auto clear_blind = [&](int i, uint32_t half) {     // by a whole warp; true
+    const int blind = -off - tile(i >> 1) * kTile - (i & 1) * kHalf;
+    if (z.causal && blind > 0) zero_rows<D>(half, kChunk, 0, min(kHalf, blind));
+    return true;
+  };
 
   if (warp == kTmaWarp) {
     // ------------------------------------------------------------ TMA producer: a half of q with lse2 and delta, that of dout, ...
@@ -249,47 +260,53 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
     }
   } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issuer
+    // ------------------------------------------------------------ MMA issuer of S^T and dV
     // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
-    // share with others their rows are cleared, so that whatever q and dout hold there meets a probability of 0 as 0.
-    auto arrived = [&](int i, bool grad) {
-      const int s = i % C::kSlots;
-      if (!warp_wait(grad ? m.full2(s) : m.full(s), (i / C::kSlots) & 1, &abort_flag)) return false;
-      const int blind = -off - tile(i >> 1) * kTile - (i & 1) * kHalf;
-      if (z.causal && blind > 0) zero_rows<D>(grad ? m.g(s) : m.q(s), kChunk, 0, min(kHalf, blind));
-      tc_fence_after();
-      return true;
-    };
+    // share with others their rows are cleared, so that whatever q and dout hold there meets a probability of 0 as 0 (the scores
+    // themselves are masked; both warps clear the rows of dout, with the same zeros).
     auto scores = [&](int i) {             // S^T of half i
-      if (!arrived(i, false)) return false;
-      product_ss<D, kHalf>(tmem + C::kS + (i & 1) * kHalf, m.fixed(0), m.q(i % C::kSlots), kChunk);
+      const int s = i % C::kSlots;
+      if (!warp_wait(m.full(s), (i / C::kSlots) & 1, &abort_flag)) return false;
+      tc_fence_after();
+      product_ss<D, kHalf>(tmem + C::kS + (i & 1) * kHalf, m.fixed(0), m.q(s), kChunk);
       tc_commit_warp(m.bar(kSFull + (i & 1)));
       return true;
     };
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && scores(1);
+    for (int i = 0; i < 2 * count && ok; ++i) {      // half i's probabilities are ready: dV += P^T dO, the scores of the half after next
+      const int s = i % C::kSlots;
+      ok = warp_wait(m.full2(s), (i / C::kSlots) & 1, &abort_flag) && clear_blind(i, m.g(s)) &&
+           warp_wait(m.bar(kPReady + (i & 1)), (i >> 1) & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      product_ts<D>(tmem + C::kAcc0, tmem + C::kS + (i & 1) * kHalf, m.g(s), kChunk, kHalf / 16, i > 0);
+      tc_commit_warp(m.empty2(s));
+      if (i + 2 < 2 * count) ok = scores(i + 2);
+    }
+    if (ok && count > 0) tc_commit_warp(m.bar(kDone));
+  } else if (warp == kMmaWarp + 1) {
+    // ------------------------------------------------------------ MMA issuer of dP^T and dK
     auto gradients = [&](int i) {          // dP^T of half i
-      if (!arrived(i, true)) return false;
-      product_ss<D, kHalf>(tmem + C::kDp + (i & 1) * kHalf, m.fixed(1), m.g(i % C::kSlots), kChunk);
+      const int s = i % C::kSlots;
+      if (!warp_wait(m.full2(s), (i / C::kSlots) & 1, &abort_flag) || !clear_blind(i, m.g(s))) return false;
+      tc_fence_after();
+      product_ss<D, kHalf>(tmem + C::kDp + (i & 1) * kHalf, m.fixed(1), m.g(s), kChunk);
       tc_commit_warp(m.bar(kDpFull + (i & 1)));
+      tc_commit_warp(m.empty2(s));
       return true;
     };
-    auto add_dv = [&](int i) {             // half i's probabilities are ready: dV += P^T dO, then the scores of the half after next
-      if (!warp_wait(m.bar(kPReady + (i & 1)), (i >> 1) & 1, &abort_flag)) return false;
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && gradients(0) && gradients(1);
+    for (int i = 0; i < 2 * count && ok; ++i) {      // half i's dS is ready: dK += dS^T Q, dP of the half after next
+      const int s = i % C::kSlots;
+      ok = warp_wait(m.full(s), (i / C::kSlots) & 1, &abort_flag) && clear_blind(i, m.q(s)) &&
+           warp_wait(m.bar(kDsReady + (i & 1)), (i >> 1) & 1, &abort_flag);
+      if (!ok) break;
       tc_fence_after();
-      product_ts<D>(tmem + C::kAcc0, tmem + C::kS + (i & 1) * kHalf, m.g(i % C::kSlots), kChunk, kHalf / 16, i > 0);
-      tc_commit_warp(m.empty2(i % C::kSlots));
-      return i + 2 >= 2 * count || scores(i + 2);
-    };
-    auto add_dk = [&](int i) {             // half i's dS is ready: dK += dS^T Q, then dP of the half after next
-      if (!warp_wait(m.bar(kDsReady + (i & 1)), (i >> 1) & 1, &abort_flag)) return false;
-      tc_fence_after();
-      product_ts<D>(tmem + C::kAcc1, tmem + C::kDp + (i & 1) * kHalf, m.q(i % C::kSlots), kChunk, kHalf / 16, i > 0);
-      tc_commit_warp(m.empty(i % C::kSlots));
-      return i + 2 >= 2 * count || gradients(i + 2);
-    };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0) && scores(1) && gradients(1);
-    // half a turn apart: P of one half gets ready with dS of the other
-    for (int i = 0; i < 2 * count && ok; ++i) ok = add_dv(i) && (i == 0 || add_dk(i - 1));
-    if (ok && add_dk(2 * count - 1)) tc_commit_warp(m.bar(kDone));
+      product_ts<D>(tmem + C::kAcc1, tmem + C::kDp + (i & 1) * kHalf, m.q(s), kChunk, kHalf / 16, i > 0);
+      tc_commit_warp(m.empty(s));
+      if (i + 2 < 2 * count) ok = gradients(i + 2);
+    }
+    if (ok && count > 0) tc_commit_warp(m.bar(kDone));
   } else {
     // ------------------------------------------------------------ probabilities: thread = key; half g, 32 queries of it
     const int g = warp >> 3, w = (warp >> 2) & 1, row = k0 + (threadIdx.x & 127);
@@ -383,7 +400,7 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (m.bar(10) - m.base));
   uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (m.bar(11) - m.base));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  setup<D>(m, &abort_flag, &tmem_slot, warp);
+  setup<D, false>(m, &abort_flag, &tmem_slot, warp);
   constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
@@ -406,21 +423,23 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
       }
     }
   } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issuer
-    auto wait_stage = [&](int i) { return warp_wait(m.full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
-    auto keys_in = [&](int j) { return min(kTile, n - (j0 + j) * kTile); };
-    auto scores = [&](int j) {             // S(j) = Q K_j^T; the keys' rows behind the sample's length are cleared for dS K
-      if (!wait_stage(2 * j)) return false;
-      const int keys = keys_in(j);
-      if (keys & 15) zero_rows<D>(m.stage(2 * j % C::kStages), kChunk, keys, (keys + 15) & ~15);
+    // ------------------------------------------------------------ MMA issuer of S
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag);
+    for (int j = 0; j < count && ok; ++j) {          // S(j) = Q K_j^T, once both halves have read S(j - 2)
+      const int s = 2 * j % C::kStages;
+      ok = warp_wait(m.full(s), (2 * j / C::kStages) & 1, &abort_flag) &&
+           (j < 2 || warp_wait(m.bar(kPReady + (j & 1)), ((j >> 1) & 1) ^ 1, &abort_flag));
+      if (!ok) break;
       tc_fence_after();
-      product_ss<D, kTile>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(2 * j % C::kStages), kChunk);
+      product_ss<D, kTile>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(s), kChunk);
       tc_commit_warp(m.bar(kSFull + (j & 1)));
-      return true;
-    };
+    }
+  } else if (warp == kMmaWarp + 1) {
+    // ------------------------------------------------------------ MMA issuer of dP and dQ
+    auto keys_in = [&](int j) { return min(kTile, n - (j0 + j) * kTile); };
     auto gradients = [&](int j, int g) {   // half g of dP(j) = dO V_j^T
       const int s = (2 * j + 1) % C::kStages;
-      if (!wait_stage(2 * j + 1)) return false;
+      if (!warp_wait(m.full(s), ((2 * j + 1) / C::kStages) & 1, &abort_flag)) return false;
       tc_fence_after();
       product_ss<D, kHalf>(tmem + C::kDp + g * kHalf, m.fixed(1), m.stage(s) + g * (kHalf * 128), kChunk);
       tc_commit_warp(m.bar(kDpFull + g));
@@ -429,6 +448,10 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
     };
     auto add_dq = [&](int j, int g) {      // half g of dS(j) is ready: dQ += dS K
       const int s = 2 * j % C::kStages;
+      if (g == 0) {                        // the keys' rows behind the sample's length are cleared: S, which reads them too, is masked
+        if (!warp_wait(m.full(s), (2 * j / C::kStages) & 1, &abort_flag)) return false;
+        if (keys_in(j) & 15) zero_rows<D>(m.stage(s), kChunk, keys_in(j), (keys_in(j) + 15) & ~15);
+      }
       if (!warp_wait(m.bar(kDsReady + g), j & 1, &abort_flag)) return false;
       tc_fence_after();
       const int steps = (min(kHalf, keys_in(j) - g * kHalf) + 15) / 16;
@@ -436,12 +459,10 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
       if (g == 1) tc_commit_warp(m.empty(s));
       return true;
     };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0, 0) && gradients(0, 1) &&
-              (count == 1 || scores(1));
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && gradients(0, 0) && gradients(0, 1);
     for (int j = 0; j < count && ok; ++j) {
       const bool more = j + 1 < count;
-      ok = add_dq(j, 0) && (!more || gradients(j + 1, 0)) && add_dq(j, 1) && (!more || gradients(j + 1, 1)) &&
-           (j + 2 >= count || scores(j + 2));
+      ok = add_dq(j, 0) && (!more || gradients(j + 1, 0)) && add_dq(j, 1) && (!more || gradients(j + 1, 1));
     }
     if (ok && count > 0) tc_commit_warp(m.bar(kDone));
   } else {
@@ -461,6 +482,9 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
       uint32_t s[32], word[16];
       tc_ld32(tmem + lanes + ((j & 1) ? kS1 : C::kS) + col, s);
       tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(m.bar(kPReady + (j & 1)));
       f2 pr[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, lse), e);

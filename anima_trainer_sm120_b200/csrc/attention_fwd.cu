@@ -8,7 +8,8 @@
 //   O += P V      tcgen05 with P read from tensor memory, V as it lies (keys along rows: the MN-major form), fp32.
 // The scores of a query tile have two buffers: S of the step after next is issued behind O += P V, which frees its buffer, so
 // a warpgroup finds its next scores ready and the special-function unit, shared by both, never waits for the tensor cores.
-// One warp issues the products, one feeds tiles of 128 keys of K and V through a ring of TMA boxes.
+// A warp for each query tile issues its products (the waits of one overlap the products of the other), one feeds tiles of 128
+// keys of K and V through a ring of TMA boxes.
 // The running maximum of a row is only raised once a score exceeds it by 2^8: until then p is at most 256, which costs neither
 // bf16 (relative) nor the fp32 sums anything, and O, which lies in tensor memory, need not be rescaled.
 // Few rows (one token, a short text) leave SMs idle: the keys are then cut into ranges, whose normalised fp32 outputs and
@@ -22,15 +23,16 @@ namespace anima {
 namespace attn {
 namespace {
 
-constexpr int kThreads = 320;            // two softmax warpgroups, one MMA warp, one TMA warp
+constexpr int kThreads = 352;            // two softmax warpgroups, an MMA warp for each query tile, one TMA warp
+constexpr int kMmaWarp = 8, kTmaWarp = 10;
 constexpr int kStep = 64;                // keys of a step
 constexpr float kMaxSlack = 8.f;         // log2 of how far a score may exceed the maximum in use
-constexpr int kPoly = 0;                 // of four pairs of exponentials, those made on the multiply-add pipes
+constexpr int kPoly = 1;                 // of four pairs of exponentials, those made on the multiply-add pipes
 
 template <int D>
 struct FwdCfg {
   static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kBars = 2 * kStages + 13;
+  static constexpr int kBars = 2 * kStages + 14;
   static constexpr int kSmem = (2 + kStages) * static_cast<int>(tile_bytes<D>()) + kBars * 8;
   static_assert(kSmem <= 227 * 1024 - 16, "shared memory");
   // tensor-memory columns: scores of tile t, buffer x at 128 t + 64 x
@@ -70,17 +72,21 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   auto s_full = [&](int t, int x) { return q_full + 8 * (1 + 2 * t + x); };
   auto p_full = [&](int t, int x) { return q_full + 8 * (5 + 2 * t + x); };
   auto o_done = [&](int t, int x) { return q_full + 8 * (9 + 2 * t + x); };
+  const uint32_t first_done = q_full + 8 * 13;     // tile 0 is through its first softmax
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int i = 0; i < C::kBars; ++i) mbar_init(bars + 8 * i, i >= 2 * C::kStages + 5 && i < 2 * C::kStages + 9 ? 4 : 1);
+    for (int i = 0; i < C::kBars; ++i) {
+      const bool p = i >= 2 * C::kStages + 5 && i < 2 * C::kStages + 9, e = i >= C::kStages && i < 2 * C::kStages;
+      mbar_init(bars + 8 * i, p ? 4 : (e ? 2 : 1));
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
   }
-  if (warp == 8) tc_alloc(smem_u32(&tmem_slot), 512);
+  if (warp == kMmaWarp) tc_alloc(smem_u32(&tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -104,7 +110,7 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   }
   const int most = max(count[0], count[1]);
 
-  if (warp == 9) {
+  if (warp == kTmaWarp) {
     // ------------------------------------------------------------ TMA producer: K0, V0, K1, V1, ...
     if (lane == 0 && most > 0) {
       mbar_expect_tx(q_full, kBytes * (count[1] > 0 ? 2 : 1));
@@ -117,56 +123,54 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         load_rows<D, kTile>(kv_smem(s), (i & 1) ? &map_v : &map_k, full(s), k0 + (i >> 1) * kTile, hk, b);
       }
     }
-  } else if (warp == 8) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp >= kMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer of query tile t
     constexpr uint32_t kIdescS = tc_idesc_bf16(kTile, kStep), kIdescO = tc_idesc_bf16(kTile, D, true);
-    auto k_stage = [&](int u) { return (u >> 1) * 2 % C::kStages; };
-    auto v_stage = [&](int u) { return ((u >> 1) * 2 + 1) % C::kStages; };
+    const int t = warp - kMmaWarp;
+    const uint64_t q_desc = tc_desc_sw128(q_smem(t));
     auto arrived = [&](int i) { return warp_wait(full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
-    auto scores = [&](int t, int u) {          // S of query tile t and step u 
-      const uint64_t a = tc_desc_sw128(q_smem(t)), k = tc_desc_sw128(kv_smem(k_stage(u)) + (u & 1) * (kStep * 128));
+    auto scores = [&](int u) {                 // S of step u
+      const uint64_t k = tc_desc_sw128(kv_smem((u >> 1) * 2 % C::kStages) + (u & 1) * (kStep * 128));
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
         const uint32_t at = (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2;   // 16 bytes a unit
-        tc_mma_ss(tmem + C::kS + t * kTile + (u & 1) * kStep, a + at, k + at, kIdescS, i > 0);
+        tc_mma_ss(tmem + C::kS + t * kTile + (u & 1) * kStep, q_desc + at, k + at, kIdescS, i > 0);
       }
       tc_commit_warp(s_full(t, u & 1));
     };
+    // a stage is free when both tiles are through with it; a tile that takes no part in a step (causal, short) says so at once
     bool ok = most > 0 && warp_wait(q_full, 0, &abort_flag) && arrived(0);
     if (ok) {
       tc_fence_after();
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (u < count[t]) scores(t, u);
+      // half a step apart: one tile's exponentials meet the other's maxima and sums
+      if (t == 1 && count[0] > 0) ok = warp_wait(first_done, 0, &abort_flag);
+      if (count[t] > 0) scores(0);
+      if (count[t] > 1) scores(1);
       tc_commit_warp(empty(0));
     }
     for (int u = 0; u < most && ok; ++u) {
-      const int vs = v_stage(u);
-      const bool next = u + 2 < most;
-      // keys of the step that exist; the product over the others is left out, up to the next multiple of 16
-      const int keys = min(kStep, n - k0 - u * kStep), steps = (keys + 15) / 16;
-      if (!(u & 1)) ok = arrived((u >> 1) * 2 + 1) && (!next || arrived((u >> 1) * 2 + 2));
+      const int vi = (u >> 1) * 2 + 1, ki = vi + 1, vs = vi % C::kStages;
+      if (!(u & 1)) ok = arrived(vi) && (u + 2 >= most || arrived(ki));
       if (!ok) break;
-      if (keys & 15) zero_rows<D>(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128, keys, steps * 16);
-      const uint64_t v = tc_desc_sw128(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (u >= count[t]) continue;
+      if (u < count[t]) {
+        // keys of the step that exist; the product over the others is left out, up to the next multiple of 16
+        const int keys = min(kStep, n - k0 - u * kStep), steps = (keys + 15) / 16;
+        if (keys & 15) zero_rows<D>(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128, keys, steps * 16);   // by either warp: the same zeros
+        const uint64_t v = tc_desc_sw128(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128);
         ok = warp_wait(p_full(t, u & 1), (u >> 1) & 1, &abort_flag);
         if (!ok) break;
         tc_fence_after();
+        if (t == 0 && u == 0 && lane == 0) mbar_arrive(first_done);
         const uint32_t o = tmem + C::kO + t * D, pr = tmem + C::kS + t * kTile + (u & 1) * kStep;
 #pragma unroll
         for (int i = 0; i < kStep / 16; ++i)
           if (i < steps) tc_mma_ts(o, pr + i * 8, v + i * (16 * 128 / 16), kIdescO, u > 0 || i > 0);
         tc_commit_warp(o_done(t, u & 1));
-        if (u + 2 < count[t]) scores(t, u + 2);
+        if (u + 2 < count[t]) scores(u + 2);
       }
-      if (ok && (u & 1)) {
+      if (u & 1) {
         tc_commit_warp(empty(vs));
-        if (next) tc_commit_warp(empty(k_stage(u + 2)));
+        if (u + 2 < most) tc_commit_warp(empty(ki % C::kStages));
       }
     }
   } else {
@@ -178,7 +182,8 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     const int lim = key_limit(z, n, row);
     // the warp's first row sees the fewest keys: steps that end before that need no mask
     const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
-    float m = -INFINITY, l = 0.f, used = 0.f;      // maximum in use (raw scores), sum, m * c (0 while there is none)
+    float m = -INFINITY, used = 0.f;     // maximum in use (raw scores), m * c (0 while there is none)
+    f2 sum[4] = {0ull, 0ull, 0ull, 0ull};
     bool ok = true;
     for (int u = 0; u < count[t]; ++u) {
       const uint32_t at = s_at + (u & 1) * kStep;
@@ -208,7 +213,8 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         const float f = grow ? exp2_approx((m - top) * p.c) : 1.f;      // 0 where there was no maximum yet
         if (grow) {
           m = top;
-          l *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = f2_mul(sum[i], f2_dup(f));
           used = m * p.c;
         }
         if (u > 0) {                       // the product of the step before is the last one under way: S(u) came behind the others
@@ -227,7 +233,7 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
       }
       const f2 c2 = f2_dup(p.c), u2 = f2_dup(-used);
-      f2 sum[4] = {0ull, 0ull, 0ull, 0ull}, y[32];
+      f2 y[32];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t w[16];
@@ -246,13 +252,13 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       // the row's sum, behind what the tensor cores wait for
 #pragma unroll
       for (int e = 0; e < 32; ++e) sum[e & 3] = f2_add(sum[e & 3], y[e]);
-      l += f2_sum(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])));
     }
     // ------------------------------------------------------------ epilogue
     if (ok && count[t] > 0) {
       ok = warp_wait(o_done(t, (count[t] - 1) & 1), ((count[t] - 1) >> 1) & 1, &abort_flag);
       tc_fence_after();
     }
+    const float l = f2_sum(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])));
     const float inv = l == 0.f ? 0.f : 1.f / l;        // a row without keys has no sum
     const bool live = row < z.lq && ok;
     const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * z.lq + row;
@@ -308,7 +314,7 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kMmaWarp) {
     tc_fence_after();
     tc_dealloc(tmem, 512);
   }
