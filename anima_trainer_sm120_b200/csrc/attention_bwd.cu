@@ -13,10 +13,11 @@
 // whose order would change results, and 4 bytes a key tile and element of traffic), and the sums stay in tensor memory.
 // Each tile of q, dO, K lies in shared memory once and serves as a K-major operand of one product and as an MN-major operand
 // of another.
-// A query tile (keys kernel) or key tile (queries kernel) is taken in two halves of 64, each with tensor memory, barriers and two
-// of the four warpgroups of its own: while one half makes exponentials, the other makes dS, and the tensor cores work on what
-// either has finished. Two warps issue the products (keys: one S and dV, one dP and dK; queries: one S, one dP and dQ), so that
-// the waits of one overlap the products of the other.
+// Four warpgroups share a pair of tiles, 32 columns each. One warp issues all products, in the order in which they are waited for
+// (a second one lets dK run between dV and the next S, which all warpgroups wait for: 3000 instead of 2600 cycles a pair): dV(i)
+// and S(i+1) as soon as P(i) lies in tensor memory, dK(i) and dP(i+1) as soon as dS(i) does.
+// Products of 64 instead of 128 columns would let the halves of a tile take turns, but read their A operand from shared memory
+// twice as often, which then bounds them (1.5 x the time of the same work in whole tiles).
 // Bound: 14 D flop a (query, key) pair on the tensor cores; two exponentials.
 #include "attention_common.cuh"
 
@@ -24,10 +25,9 @@ namespace anima {
 namespace attn {
 namespace {
 
-constexpr int kWorkers = 16;             // warps that make probabilities: two warpgroups for each half of a tile
-constexpr int kMmaWarp = kWorkers, kTmaWarp = kWorkers + 2, kThreads = (kWorkers + 3) * 32;   // two warps issue products
-constexpr int kHalf = kTile / 2;
-constexpr int kPoly = 0;                 // of four pairs of exponentials, those made on the multiply-add pipes
+constexpr int kWorkers = 16;             // warps that make probabilities: four warpgroups
+constexpr int kMmaWarp = kWorkers, kTmaWarp = kWorkers + 1, kThreads = (kWorkers + 2) * 32;
+constexpr int kPoly = 1;                 // of four pairs of exponentials, those made on the multiply-add pipes
 
 struct BwdParams {
   Sizes z;
@@ -79,17 +79,15 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
   p.delta[to] = lse == -INFINITY ? 0.f : -s;
 }
 
-// Shared memory: two tiles that stay, a ring (keys: half tiles of q with their lse2 and delta, and of dout; queries: tiles of K
+// Shared memory: two tiles that stay, a ring (keys: three tiles of q, two of dout with lse2 and delta; queries: five tiles of K
 // and V), barriers.
 template <int D>
 struct BwdCfg {
-  static constexpr uint32_t kBytes = tile_bytes<D>(), kHalfBytes = kBytes / 2;
-  static constexpr int kSlots = 5;                                     // half tiles of q, and of dout
-  static constexpr int kRowBytes = 2 * kHalf * 4;                      // lse2 and delta of a half
-  static constexpr int kStages = 5;                                    // tiles of K or V
-  static constexpr int kBars = 4 * kSlots + 12;
-  static constexpr int kSmem = 2 * kBytes + kSlots * (2 * kHalfBytes + kRowBytes) + kBars * 8;
-  static_assert(kSlots * 2 * kHalfBytes >= kStages * kBytes, "one size for both kernels");
+  static constexpr uint32_t kBytes = tile_bytes<D>();
+  static constexpr int kQ = 3, kG = 2, kStages = kQ + kG;              // tiles of q, of dout; of K and V
+  static constexpr int kRowBytes = 2 * kTile * 4;                      // lse2 and delta of a tile
+  static constexpr int kBars = 12 + 2 * kStages;
+  static constexpr int kSmem = (2 + kStages) * kBytes + kG * kRowBytes + kBars * 8;
   static_assert(kSmem <= 227 * 1024, "shared memory");
   static constexpr uint32_t kS = 0, kDp = 128, kAcc0 = 256, kAcc1 = 256 + D;   // tensor-memory columns
 };
@@ -98,30 +96,23 @@ struct Layout {
   using C = BwdCfg<D>;
   uint32_t base;
   __device__ __forceinline__ uint32_t fixed(int i) const { return base + i * C::kBytes; }
-  __device__ __forceinline__ uint32_t ring() const { return base + 2 * C::kBytes; }
-  __device__ __forceinline__ uint32_t stage(int s) const { return ring() + s * C::kBytes; }                            // queries
-  __device__ __forceinline__ uint32_t q(int s) const { return ring() + s * C::kHalfBytes; }                            // keys
-  __device__ __forceinline__ uint32_t g(int s) const { return ring() + (C::kSlots + s) * C::kHalfBytes; }
-  __device__ __forceinline__ uint32_t row_data(int s) const { return ring() + 2 * C::kSlots * C::kHalfBytes + s * C::kRowBytes; }
-  __device__ __forceinline__ uint32_t bar(int i) const { return row_data(C::kSlots) + 8 * i; }     // 10, 11: the abort flag, the tensor-memory address
+  __device__ __forceinline__ uint32_t stage(int s) const { return base + (2 + s) * C::kBytes; }        // keys: those of dout come first
+  __device__ __forceinline__ uint32_t row_data(int s) const { return base + (2 + C::kStages) * C::kBytes + s * C::kRowBytes; }
+  __device__ __forceinline__ uint32_t bar(int i) const { return row_data(C::kG) + 8 * i; }             // 10, 11: the abort flag, the tensor-memory address
   __device__ __forceinline__ uint32_t full(int s) const { return bar(12 + s); }
-  __device__ __forceinline__ uint32_t empty(int s) const { return bar(12 + C::kSlots + s); }
-  __device__ __forceinline__ uint32_t full2(int s) const { return bar(12 + 2 * C::kSlots + s); }
-  __device__ __forceinline__ uint32_t empty2(int s) const { return bar(12 + 3 * C::kSlots + s); }
+  __device__ __forceinline__ uint32_t empty(int s) const { return bar(12 + C::kStages + s); }
 };
-// one barrier each, or one for each half (or score buffer)
+// (queries: kSFull one for each score buffer)
 enum { kFixedFull = 0, kDone = 1, kSFull = 2, kDpFull = 4, kPReady = 6, kDsReady = 8 };
 
-template <int D, bool KEYS>
+template <int D>
 __device__ __forceinline__ void setup(const Layout<D>& m, volatile int* abort_flag, uint32_t* tmem_slot, int warp) {
   using C = BwdCfg<D>;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < C::kBars; ++i) {
       int arrivals = 1;
-      if (i >= kPReady && i < kPReady + 2) arrivals = KEYS ? kWorkers / 2 : kWorkers;      // queries: S(j) has been read
-      if (i >= kDsReady && i < kDsReady + 2) arrivals = kWorkers / 2;
-      if (KEYS && (i == kDone || i >= 12 + 3 * C::kSlots)) arrivals = 2;                   // both MMA warps
+      if (i >= kPReady && i < kDsReady + 2) arrivals = kWorkers;
       if (i < 10 || i >= 12) mbar_init(m.bar(i), arrivals);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -147,21 +138,23 @@ __device__ __forceinline__ void teardown(volatile int* abort_flag, int32_t* stat
   }
 }
 
-// D[tmem] = A . B^T: A a tile of 128 rows, B of N rows whose 64-column chunks lie b_chunk bytes apart, the head vector along K
-template <int D, int N>
-__device__ __forceinline__ void product_ss(uint32_t d, uint32_t a_smem, uint32_t b_smem, uint32_t b_chunk) {
+// D[tmem] = A . B^T of two tiles in shared memory, the head vector along K
+template <int D>
+__device__ __forceinline__ void product_ss(uint32_t d, uint32_t a_smem, uint32_t b_smem) {
   const uint64_t a = tc_desc_sw128(a_smem), b = tc_desc_sw128(b_smem);
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)      // 16 bytes a unit
-    tc_mma_ss(d, a + (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2, b + (i >> 2) * (b_chunk / 16) + (i & 3) * 2, tc_idesc_bf16(kTile, N), i > 0);
+  for (int i = 0; i < D / 16; ++i) {
+    const uint32_t at = (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2;     // 16 bytes a unit
+    tc_mma_ss(d, a + at, b + at, tc_idesc_bf16(kTile, kTile), i > 0);
+  }
 }
-// D[tmem] += A . B over 16 `steps` (at most 4) rows of B (64-column chunks b_chunk bytes apart): A bf16 in tensor memory, elements 32 w .. 32 w + 31
-// of a row in columns a + 32 w .. + 15
+// D[tmem] += A . B over the first 16 `steps` rows of the tile B: A bf16 in tensor memory, elements 32 w .. 32 w + 31 of a row in
+// columns a + 32 w .. + 15
 template <int D>
-__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b_smem, uint32_t b_chunk, int steps, bool accumulate) {
-  const uint64_t b = tc_desc_sw128(b_smem, b_chunk);
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b_smem, int steps, bool accumulate) {
+  const uint64_t b = tc_desc_sw128(b_smem, kTile * 128);
 #pragma unroll
-  for (int i = 0; i < kHalf / 16; ++i)
+  for (int i = 0; i < kTile / 16; ++i)
     if (i < steps) tc_mma_ts(d, a + (i >> 1) * 32 + (i & 1) * 8, b + i * (16 * 128 / 16), tc_idesc_bf16(kTile, D, true), accumulate || i > 0);
 }
 
@@ -214,13 +207,12 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                           const __grid_constant__ BwdParams p) {
   using C = BwdCfg<D>;
-  constexpr uint32_t kChunk = kHalf * 128;     // bytes of 64 rows of a 64-column chunk
   extern __shared__ __align__(1024) uint8_t smem[];
   const Layout<D> m{smem_u32(smem)};
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (m.bar(10) - m.base));
   uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (m.bar(11) - m.base));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  setup<D, true>(m, &abort_flag, &tmem_slot, warp);
+  setup<D>(m, &abort_flag, &tmem_slot, warp);
   constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
@@ -230,99 +222,87 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const int first = z.causal ? min(q_tiles, max(0, k0 - off) / kTile) : 0;     // the first query tile with a row that sees a key here
   const int per_head = k0 < n ? q_tiles - first : 0;
   const int begin = split * p.per_split, count = max(0, min(z.group * per_head, begin + p.per_split) - begin);
-  // pass i of this CTA: query tile `tile(i)` of head `head(i)`; its halves are 2 i and 2 i + 1
+  // pass i of this CTA: query tile `tile(i)` of head `head(i)`
   auto head = [&](int i) { return hk * z.group + (begin + i) / per_head; };
   auto tile = [&](int i) { return first + (begin + i) % per_head; };
-  auto clear_blind = [&](int i, uint32_t half) {     // by a whole warp; true
-    const int blind = -off - tile(i >> 1) * kTile - (i & 1) * kHalf;
-    if (z.causal && blind > 0) zero_rows<D>(half, kChunk, 0, min(kHalf, blind));
+  // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
+  // share with others their rows of q and dout are cleared (by a whole warp), so that whatever they hold meets a probability of
+  // 0 as 0.
+  auto clear_blind = [&](int i, uint32_t at) {
+    const int blind = -off - tile(i) * kTile;
+    if (z.causal && blind > 0) zero_rows<D>(at, kTile * 128, 0, min(kTile, blind));
     return true;
   };
+  auto g_at = [](int i) { return i % C::kG; };
+  auto q_at = [](int i) { return C::kG + i % C::kQ; };
 
   if (warp == kTmaWarp) {
-    // ------------------------------------------------------------ TMA producer: a half of q with lse2 and delta, that of dout, ...
+    // ------------------------------------------------------------ TMA producer: q0, dout0 (with lse2, delta), q1, ...
     if (lane == 0 && count > 0) {
       mbar_expect_tx(m.bar(kFixedFull), 2 * C::kBytes);
       load_rows<D, kTile>(m.fixed(0), &map_k, m.bar(kFixedFull), k0, hk, b);
       load_rows<D, kTile>(m.fixed(1), &map_v, m.bar(kFixedFull), k0, hk, b);
-      for (int i = 0; i < 2 * count; ++i) {
-        const int s = i % C::kSlots, h = head(i >> 1), q0 = tile(i >> 1) * kTile + (i & 1) * kHalf;
-        const uint32_t phase = ((i / C::kSlots) & 1) ^ 1;
-        if (!mbar_wait(m.empty(s), phase, &abort_flag)) break;
-        mbar_expect_tx(m.full(s), C::kHalfBytes + C::kRowBytes);
-        load_rows<D, kHalf>(m.q(s), &map_q, m.full(s), q0, h, b);
+      for (int i = 0; i < count; ++i) {
+        const int s = q_at(i), r = g_at(i), h = head(i), q0 = tile(i) * kTile;
+        if (!mbar_wait(m.empty(s), ((i / C::kQ) & 1) ^ 1, &abort_flag)) break;
+        mbar_expect_tx(m.full(s), C::kBytes);
+        load_rows<D, kTile>(m.stage(s), &map_q, m.full(s), q0, h, b);
+        if (!mbar_wait(m.empty(r), ((i / C::kG) & 1) ^ 1, &abort_flag)) break;
+        mbar_expect_tx(m.full(r), C::kBytes + C::kRowBytes);
         const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + q0;
-        bulk_load(m.row_data(s), p.lse2 + at, kHalf * 4, m.full(s));
-        bulk_load(m.row_data(s) + kHalf * 4, p.delta + at, kHalf * 4, m.full(s));
-        if (!mbar_wait(m.empty2(s), phase, &abort_flag)) break;
-        mbar_expect_tx(m.full2(s), C::kHalfBytes);
-        load_rows<D, kHalf>(m.g(s), &map_do, m.full2(s), q0, h, b);
+        bulk_load(m.row_data(r), p.lse2 + at, kTile * 4, m.full(r));
+        bulk_load(m.row_data(r) + kTile * 4, p.delta + at, kTile * 4, m.full(r));
+        load_rows<D, kTile>(m.stage(r), &map_do, m.full(r), q0, h, b);
       }
     }
   } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issuer of S^T and dV
-    // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
-    // share with others their rows are cleared, so that whatever q and dout hold there meets a probability of 0 as 0 (the scores
-    // themselves are masked; both warps clear the rows of dout, with the same zeros).
-    auto scores = [&](int i) {             // S^T of half i
-      const int s = i % C::kSlots;
-      if (!warp_wait(m.full(s), (i / C::kSlots) & 1, &abort_flag)) return false;
+    // ------------------------------------------------------------ MMA issuer
+    auto scores = [&](int i) {             // S^T(i) = K Q^T
+      if (!warp_wait(m.full(q_at(i)), (i / C::kQ) & 1, &abort_flag) || !clear_blind(i, m.stage(q_at(i)))) return false;
       tc_fence_after();
-      product_ss<D, kHalf>(tmem + C::kS + (i & 1) * kHalf, m.fixed(0), m.q(s), kChunk);
-      tc_commit_warp(m.bar(kSFull + (i & 1)));
+      product_ss<D>(tmem + C::kS, m.fixed(0), m.stage(q_at(i)));
+      tc_commit_warp(m.bar(kSFull));
       return true;
     };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && scores(1);
-    for (int i = 0; i < 2 * count && ok; ++i) {      // half i's probabilities are ready: dV += P^T dO, the scores of the half after next
-      const int s = i % C::kSlots;
-      ok = warp_wait(m.full2(s), (i / C::kSlots) & 1, &abort_flag) && clear_blind(i, m.g(s)) &&
-           warp_wait(m.bar(kPReady + (i & 1)), (i >> 1) & 1, &abort_flag);
-      if (!ok) break;
+    auto gradients = [&](int i) {          // dP^T(i) = V dO^T
+      if (!warp_wait(m.full(g_at(i)), (i / C::kG) & 1, &abort_flag) || !clear_blind(i, m.stage(g_at(i)))) return false;
       tc_fence_after();
-      product_ts<D>(tmem + C::kAcc0, tmem + C::kS + (i & 1) * kHalf, m.g(s), kChunk, kHalf / 16, i > 0);
-      tc_commit_warp(m.empty2(s));
-      if (i + 2 < 2 * count) ok = scores(i + 2);
-    }
-    if (ok && count > 0) tc_commit_warp(m.bar(kDone));
-  } else if (warp == kMmaWarp + 1) {
-    // ------------------------------------------------------------ MMA issuer of dP^T and dK
-    auto gradients = [&](int i) {          // dP^T of half i
-      const int s = i % C::kSlots;
-      if (!warp_wait(m.full2(s), (i / C::kSlots) & 1, &abort_flag) || !clear_blind(i, m.g(s))) return false;
-      tc_fence_after();
-      product_ss<D, kHalf>(tmem + C::kDp + (i & 1) * kHalf, m.fixed(1), m.g(s), kChunk);
-      tc_commit_warp(m.bar(kDpFull + (i & 1)));
-      tc_commit_warp(m.empty2(s));
+      product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage(g_at(i)));
+      tc_commit_warp(m.bar(kDpFull));
       return true;
     };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && gradients(0) && gradients(1);
-    for (int i = 0; i < 2 * count && ok; ++i) {      // half i's dS is ready: dK += dS^T Q, dP of the half after next
-      const int s = i % C::kSlots;
-      ok = warp_wait(m.full(s), (i / C::kSlots) & 1, &abort_flag) && clear_blind(i, m.q(s)) &&
-           warp_wait(m.bar(kDsReady + (i & 1)), (i >> 1) & 1, &abort_flag);
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0);
+    for (int i = 0; i < count && ok; ++i) {
+      const bool more = i + 1 < count;
+      ok = warp_wait(m.bar(kPReady), i & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      product_ts<D>(tmem + C::kAcc1, tmem + C::kDp + (i & 1) * kHalf, m.q(s), kChunk, kHalf / 16, i > 0);
-      tc_commit_warp(m.empty(s));
-      if (i + 2 < 2 * count) ok = gradients(i + 2);
+      product_ts<D>(tmem + C::kAcc0, tmem + C::kS, m.stage(g_at(i)), kTile / 16, i > 0);
+      ok = !more || scores(i + 1);
+      ok = ok && warp_wait(m.bar(kDsReady), i & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      tc_commit_warp(m.empty(g_at(i)));    // dV(i) and dP(i) are through with it, and delta has been read
+      product_ts<D>(tmem + C::kAcc1, tmem + C::kDp, m.stage(q_at(i)), kTile / 16, i > 0);
+      tc_commit_warp(m.empty(q_at(i)));
+      ok = !more || gradients(i + 1);
     }
     if (ok && count > 0) tc_commit_warp(m.bar(kDone));
   } else {
-    // ------------------------------------------------------------ probabilities: thread = key; half g, 32 queries of it
-    const int g = warp >> 3, w = (warp >> 2) & 1, row = k0 + (threadIdx.x & 127);
+    // ------------------------------------------------------------ probabilities: thread = key, warpgroup w has 32 queries
+    const int w = warp >> 2, row = k0 + (threadIdx.x & 127);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + C::kS + g * kHalf + w * 32, dp_at = tmem + lanes + C::kDp + g * kHalf + w * 32;
+    const uint32_t s_at = tmem + lanes + C::kS + w * 32, dp_at = tmem + lanes + C::kDp + w * 32;
     const bool row_ok = row < n;
     bool ok = true;
     const f2 c2 = f2_dup(p.c);
     for (int i = 0; i < count; ++i) {
-      const int slot = (2 * i + g) % C::kSlots;
-      const uint32_t rows = m.row_data(slot) + w * 128;
+      const uint32_t rows = m.row_data(g_at(i)) + w * 128;
       // queries of these 32 before `from` do not see this key
       int from = row_ok ? 0 : 32;
-      if (z.causal && row_ok) from = row - off - tile(i) * kTile - g * kHalf - w * 32;
+      if (z.causal && row_ok) from = row - off - tile(i) * kTile - w * 32;
       const bool edge = __any_sync(0xffffffffu, from > 0);
-      ok = warp_wait(m.full(slot), ((2 * i + g) / C::kSlots) & 1, &abort_flag) && warp_wait(m.bar(kSFull + g), i & 1, &abort_flag);
+      ok = warp_wait(m.full(g_at(i)), (i / C::kG) & 1, &abort_flag) && warp_wait(m.bar(kSFull), i & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
       uint32_t s[32], word[16];
@@ -346,9 +326,9 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kPReady + g));
+      if (lane == 0) mbar_arrive(m.bar(kPReady));
 
-      ok = warp_wait(m.bar(kDpFull + g), i & 1, &abort_flag);
+      ok = warp_wait(m.bar(kDpFull), i & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
       tc_ld32(dp_at, s);
@@ -356,7 +336,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         f2 d0, d1;
-        lds_pairs(rows + kHalf * 4 + e * 8, d0, d1);
+        lds_pairs(rows + kTile * 4 + e * 8, d0, d1);
         word[e] = bf16_of_f2(f2_mul(pr[e], f2_add(pair_of(s, e), d0)));
         word[e + 1] = bf16_of_f2(f2_mul(pr[e + 1], f2_add(pair_of(s, e + 1), d1)));
       }
@@ -368,17 +348,17 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kDsReady + g));
+      if (lane == 0) mbar_arrive(m.bar(kDsReady));
     }
     if (ok && count > 0) {
       ok = warp_wait(m.bar(kDone), 0, &abort_flag);
       tc_fence_after();
     }
-    // the warpgroups of half 0: the two halves of dV; of half 1: of dK
-    const int64_t at = ((static_cast<int64_t>(b) * z.lk + row) * z.kv_heads + hk) * D + w * (D / 2);
-    __nv_bfloat16* dst = g == 0 ? p.dv : p.dk;
-    float* part = g == 0 ? p.part0 : p.part1;
-    store_row<D / 2>(tmem + lanes + (g == 0 ? C::kAcc0 : C::kAcc1) + w * (D / 2), count > 0, g == 0 ? 1.f : p.scale, ok && row < z.lk,
+    // warpgroups 0 and 1: the halves of dV; 2 and 3: of dK
+    const int64_t at = ((static_cast<int64_t>(b) * z.lk + row) * z.kv_heads + hk) * D + (w & 1) * (D / 2);
+    __nv_bfloat16* dst = w < 2 ? p.dv : p.dk;
+    float* part = w < 2 ? p.part0 : p.part1;
+    store_row<D / 2>(tmem + lanes + (w < 2 ? C::kAcc0 : C::kAcc1) + (w & 1) * (D / 2), count > 0, w < 2 ? 1.f : p.scale, ok && row < z.lk,
                      dst ? dst + at : nullptr, part ? part + split * p.elements + at : nullptr);
   }
   teardown(&abort_flag, p.status, tmem, warp);
@@ -394,13 +374,12 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
                              const __grid_constant__ BwdParams p) {
   using C = BwdCfg<D>;
   constexpr uint32_t kS1 = C::kAcc1;       // second buffer of the scores
-  constexpr uint32_t kChunk = kTile * 128;
   extern __shared__ __align__(1024) uint8_t smem[];
   const Layout<D> m{smem_u32(smem)};
   volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (m.bar(10) - m.base));
   uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (m.bar(11) - m.base));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  setup<D, false>(m, &abort_flag, &tmem_slot, warp);
+  setup<D>(m, &abort_flag, &tmem_slot, warp);
   constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
@@ -423,51 +402,38 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
       }
     }
   } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ MMA issuer of S
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag);
-    for (int j = 0; j < count && ok; ++j) {          // S(j) = Q K_j^T, once both halves have read S(j - 2)
-      const int s = 2 * j % C::kStages;
-      ok = warp_wait(m.full(s), (2 * j / C::kStages) & 1, &abort_flag) &&
-           (j < 2 || warp_wait(m.bar(kPReady + (j & 1)), ((j >> 1) & 1) ^ 1, &abort_flag));
+    // ------------------------------------------------------------ MMA issuer
+    auto wait_stage = [&](int i) { return warp_wait(m.full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
+    auto scores = [&](int j) {             // S(j) = Q K_j^T; the keys' rows behind the sample's length are cleared for dS K
+      const int s = 2 * j % C::kStages, keys = min(kTile, n - (j0 + j) * kTile);
+      if (!wait_stage(2 * j)) return false;
+      if (keys & 15) zero_rows<D>(m.stage(s), kTile * 128, keys, (keys + 15) & ~15);
+      tc_fence_after();
+      product_ss<D>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(s));
+      tc_commit_warp(m.bar(kSFull + (j & 1)));
+      return true;
+    };
+    auto gradients = [&](int j) {          // dP(j) = dO V_j^T
+      if (!wait_stage(2 * j + 1)) return false;
+      tc_fence_after();
+      product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage((2 * j + 1) % C::kStages));
+      tc_commit_warp(m.bar(kDpFull));
+      tc_commit_warp(m.empty((2 * j + 1) % C::kStages));
+      return true;
+    };
+    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0) && (count == 1 || scores(1));
+    for (int j = 0; j < count && ok; ++j) {          // dS(j) is ready: dQ += dS K, the next dP, the scores after the next
+      ok = warp_wait(m.bar(kDsReady), j & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
-      product_ss<D, kTile>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(s), kChunk);
-      tc_commit_warp(m.bar(kSFull + (j & 1)));
-    }
-  } else if (warp == kMmaWarp + 1) {
-    // ------------------------------------------------------------ MMA issuer of dP and dQ
-    auto keys_in = [&](int j) { return min(kTile, n - (j0 + j) * kTile); };
-    auto gradients = [&](int j, int g) {   // half g of dP(j) = dO V_j^T
-      const int s = (2 * j + 1) % C::kStages;
-      if (!warp_wait(m.full(s), ((2 * j + 1) / C::kStages) & 1, &abort_flag)) return false;
-      tc_fence_after();
-      product_ss<D, kHalf>(tmem + C::kDp + g * kHalf, m.fixed(1), m.stage(s) + g * (kHalf * 128), kChunk);
-      tc_commit_warp(m.bar(kDpFull + g));
-      if (g == 1) tc_commit_warp(m.empty(s));
-      return true;
-    };
-    auto add_dq = [&](int j, int g) {      // half g of dS(j) is ready: dQ += dS K
-      const int s = 2 * j % C::kStages;
-      if (g == 0) {                        // the keys' rows behind the sample's length are cleared: S, which reads them too, is masked
-        if (!warp_wait(m.full(s), (2 * j / C::kStages) & 1, &abort_flag)) return false;
-        if (keys_in(j) & 15) zero_rows<D>(m.stage(s), kChunk, keys_in(j), (keys_in(j) + 15) & ~15);
-      }
-      if (!warp_wait(m.bar(kDsReady + g), j & 1, &abort_flag)) return false;
-      tc_fence_after();
-      const int steps = (min(kHalf, keys_in(j) - g * kHalf) + 15) / 16;
-      product_ts<D>(tmem + C::kAcc0, tmem + C::kDp + g * kHalf, m.stage(s) + g * (kHalf * 128), kChunk, steps, j > 0 || g > 0);
-      if (g == 1) tc_commit_warp(m.empty(s));
-      return true;
-    };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && gradients(0, 0) && gradients(0, 1);
-    for (int j = 0; j < count && ok; ++j) {
-      const bool more = j + 1 < count;
-      ok = add_dq(j, 0) && (!more || gradients(j + 1, 0)) && add_dq(j, 1) && (!more || gradients(j + 1, 1));
+      product_ts<D>(tmem + C::kAcc0, tmem + C::kDp, m.stage(2 * j % C::kStages), (min(kTile, n - (j0 + j) * kTile) + 15) / 16, j > 0);
+      tc_commit_warp(m.empty(2 * j % C::kStages));
+      ok = (j + 1 >= count || gradients(j + 1)) && (j + 2 >= count || scores(j + 2));
     }
     if (ok && count > 0) tc_commit_warp(m.bar(kDone));
   } else {
-    // ------------------------------------------------------------ probabilities: thread = query; half g, 32 keys of it
-    const int g = warp >> 3, w = (warp >> 2) & 1, row = q0 + (threadIdx.x & 127), col = g * kHalf + w * 32;
+    // ------------------------------------------------------------ probabilities: thread = query, warpgroup w has 32 keys
+    const int w = warp >> 2, row = q0 + (threadIdx.x & 127), col = w * 32;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t dp_at = tmem + lanes + C::kDp + col;
     const int lim = key_limit(z, n, row);
@@ -482,13 +448,10 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
       uint32_t s[32], word[16];
       tc_ld32(tmem + lanes + ((j & 1) ? kS1 : C::kS) + col, s);
       tc_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kPReady + (j & 1)));
       f2 pr[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, lse), e);
-      ok = warp_wait(m.bar(kDpFull + g), j & 1, &abort_flag);
+      ok = warp_wait(m.bar(kDpFull), j & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
       tc_ld32(dp_at, s);
@@ -506,16 +469,15 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kDsReady + g));
+      if (lane == 0) mbar_arrive(m.bar(kDsReady));
     }
     if (ok && count > 0) {
       ok = warp_wait(m.bar(kDone), 0, &abort_flag);
       tc_fence_after();
     }
-    const int quarter = warp >> 2;
-    const int64_t dense = ((static_cast<int64_t>(b) * z.heads + h) * z.lq + row) * D + quarter * (D / 4);
-    store_row<D / 4>(tmem + lanes + C::kAcc0 + quarter * (D / 4), count > 0, p.scale, ok && row < z.lq,
-                     p.dq + b * p.sdq.b + row * p.sdq.l + h * p.sdq.h + quarter * (D / 4),
+    const int64_t dense = ((static_cast<int64_t>(b) * z.heads + h) * z.lq + row) * D + w * (D / 4);
+    store_row<D / 4>(tmem + lanes + C::kAcc0 + w * (D / 4), count > 0, p.scale, ok && row < z.lq,
+                     p.dq + b * p.sdq.b + row * p.sdq.l + h * p.sdq.h + w * (D / 4),
                      p.part0 ? p.part0 + split * p.elements + dense : nullptr);
   }
   teardown(&abort_flag, p.status, tmem, warp);
@@ -608,7 +570,7 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
     p.part0 = p.splits > 1 ? part : nullptr;
     p.part1 = p.splits > 1 ? part + p.splits * p.elements : nullptr;
     const dim3 grid(static_cast<unsigned>(ceil_div(s.lk, kTile) * p.splits), static_cast<unsigned>(s.kv_heads), static_cast<unsigned>(s.batch));
-    launch_after(attention_bwd_keys_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[4], maps[5], maps[2], maps[3], p);
+    launch_after(attention_bwd_keys_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
     ANIMA_CHECK_LAUNCH(who);
     if (p.splits > 1) {
       if (p.dv)
@@ -697,11 +659,9 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
   rows.heads = p.z.heads;
   rows.rows = s.batch * plan.lq_pad * s.heads;
   const void* stand_in = no_q ? k : q;
-  CUtensorMap maps[6];                   // whole tiles of q, dout, k, v; half tiles of q and dout
+  CUtensorMap maps[4];
   ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, stand_in) &&
                     attn::encode_heads(&maps[1], dout, sdo, s.batch, s.lq, s.heads, s.d, stand_in) &&
-                    attn::encode_heads(&maps[4], q, sq, s.batch, s.lq, s.heads, s.d, stand_in, attn::kHalf) &&
-                    attn::encode_heads(&maps[5], dout, sdo, s.batch, s.lq, s.heads, s.d, stand_in, attn::kHalf) &&
                     attn::encode_heads(&maps[2], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in) &&
                     attn::encode_heads(&maps[3], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in),
                 ANIMA_E_CUDA, "%s: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand)", who);
