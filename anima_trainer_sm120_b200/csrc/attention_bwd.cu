@@ -302,20 +302,19 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       int from = row_ok ? 0 : 32;
       if (z.causal && row_ok) from = row - off - tile(i) * kTile - w * 32;
       const bool edge = __any_sync(0xffffffffu, from > 0);
-      ok = warp_wait(m.full(g_at(i)), (i / C::kG) & 1, &abort_flag) && warp_wait(m.bar(kSFull), i & 1, &abort_flag);
+      ok = warp_wait(m.full(g_at(i)), (i / C::kG) & 1, &abort_flag);
+      if (!ok) break;
+      f2 pr[16], rd[16];                 // what does not depend on a product is read while waiting for it
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) lds_pairs(rows + e * 8, rd[e], rd[e + 1]);
+      ok = warp_wait(m.bar(kSFull), i & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
       uint32_t s[32], word[16];
       tc_ld32(s_at, s);
       tc_wait_ld();
-      f2 pr[16];
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        f2 l0, l1;
-        lds_pairs(rows + e * 8, l0, l1);
-        pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, l0), e);
-        pr[e + 1] = exp2_mixed(f2_fma(pair_of(s, e + 1), c2, l1), e + 1);
-      }
+      for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, rd[e]), e);
       if (edge) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) pr[e] = f2_make(2 * e >= from ? f2_lo(pr[e]) : 0.f, 2 * e + 1 >= from ? f2_hi(pr[e]) : 0.f);
