@@ -3,9 +3,9 @@
 // Three launches, no atomics, every sum in a fixed order:
 //   rows   -delta = -out . dout of each query, and minus its log-sum in base 2 (-inf for a query that saw nothing, and for the
 //          rows that fill up the last tile: their probabilities come out as 0);
-//   keys   one CTA a tile of 128 keys of a key head walks the query tiles of all heads it serves:
+//   keys   a CTA takes tiles of 128 keys of a key head and walks, for each, the query tiles of all heads it serves:
 //            S^T = K Q^T, dP^T = V dO^T (lane = key, column = query), dV += P^T dO, dK += dS^T Q;
-//   queries one CTA a tile of 128 queries of a head walks the key tiles:
+//   queries a CTA takes tiles of 128 queries of a head and walks the key tiles for each:
 //            S = Q K^T, dP = dO V^T (lane = query), dQ += dS K.
 // That is 7 products a pair of tiles where one kernel for all three would do 5. It buys this: P^T, dS^T and dS are read by the
 // tensor cores from tensor memory, where the threads that made them wrote them over the scores, and never cross shared memory
@@ -36,7 +36,8 @@ struct BwdParams {
   int lq_pad;
   __nv_bfloat16 *dq, *dk, *dv;
   Strided sdq;                           // dk, dv: dense
-  int splits, per_split;                 // ranges of query tiles (keys) or key tiles (queries) a CTA takes
+  int tiles, splits, per_split;          // key (query) tiles; ranges their walks are cut into, and how long these are
+  int items;                             // tiles * splits * heads * batch
   float *part0, *part1;                  // fp32 partial sums [split][elements], if splits > 1: dv and dk, or dq
   int64_t elements;
   int32_t* status;
@@ -103,18 +104,41 @@ struct Layout {
   __device__ __forceinline__ uint32_t empty(int s) const { return bar(12 + C::kStages + s); }
 };
 // (queries: kSFull one for each score buffer)
-enum { kFixedFull = 0, kDone = 1, kSFull = 2, kDpFull = 4, kPReady = 6, kDsReady = 8 };
+enum { kFixedFull = 0, kDone = 1, kSFull = 2, kDpFull = 4, kAccFree = 5, kPReady = 6, kFixedFree = 7, kDsReady = 8 };
+
+// One item of a CTA's work: range `split` of the walk of one tile. The CTAs go through the items in turn, so that the loads and
+// first products of an item overlap the last passes and the way out of the one before. Causal, the tiles' walks differ in
+// length: their order turns by one from head to head, or a CTA would meet the same ones again and again. 32-bit arithmetic: a
+// 64-bit division is a call, behind which the compiler takes nothing for uniform any more (see phase_of; 761 became 873 us).
+struct Item {
+  int split, tile, head, b;
+};
+// Every item takes the stages of a ring from the first on, so that where a pass finds its operands follows from its number in
+// the item alone, which the compiler keeps in uniform registers (with stages counted through all items the products' descriptors
+// went through ordinary ones: 72 instead of 20 cycles an instruction). What carries over from item to item, the phases of the
+// barriers, is one bit each.
+__device__ __forceinline__ uint32_t phase_of(uint32_t& bits, int s) {      // of the next completion of barrier s
+  const uint32_t now = (bits >> s) & 1u;
+  bits ^= 1u << s;
+  return now;
+}
+__device__ __forceinline__ Item item_of(const BwdParams& p, int id, int heads) {
+  Item it;
+  it.split = id % p.splits;
+  const int rest = id / p.splits, bh = rest / p.tiles;
+  it.tile = (rest + (p.z.causal ? bh % p.tiles : 0)) % p.tiles;
+  it.head = bh % heads;
+  it.b = bh / heads;
+  return it;
+}
 
 template <int D>
 __device__ __forceinline__ void setup(const Layout<D>& m, volatile int* abort_flag, uint32_t* tmem_slot, int warp) {
   using C = BwdCfg<D>;
   if (threadIdx.x == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < C::kBars; ++i) {
-      int arrivals = 1;
-      if (i >= kPReady && i < kDsReady + 2) arrivals = kWorkers;
-      if (i < 10 || i >= 12) mbar_init(m.bar(i), arrivals);
-    }
+    for (int i = 0; i < C::kBars; ++i)
+      if (i < 10 || i >= 12) mbar_init(m.bar(i), i == kAccFree || i == kPReady || i == kDsReady ? kWorkers : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) tc_alloc(smem_u32(tmem_slot), 512);
@@ -200,7 +224,6 @@ __device__ __forceinline__ f2 pair_of(const uint32_t (&v)[32], int e) { return f
 __device__ __forceinline__ f2 exp2_mixed(f2 x, int e) { return (e & 3) < kPoly ? exp2_poly(x) : exp2_pair(x); }
 
 // ------------------------------------------------------------------------------------------------ keys: dK, dV
-// grid (key tiles * splits, kv_heads, batch)
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
@@ -216,155 +239,198 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
-  const int split = blockIdx.x % p.splits, jt = blockIdx.x / p.splits, hk = blockIdx.y, b = blockIdx.z;
-  const int k0 = jt * kTile, n = keys_of(z, b), off = z.lk - z.lq;
-  const int q_tiles = (z.lq + kTile - 1) / kTile;
-  const int first = z.causal ? min(q_tiles, max(0, k0 - off) / kTile) : 0;     // the first query tile with a row that sees a key here
-  const int per_head = k0 < n ? q_tiles - first : 0;
-  const int begin = split * p.per_split, count = max(0, min(z.group * per_head, begin + p.per_split) - begin);
-  // pass i of this CTA: query tile `tile(i)` of head `head(i)`
-  auto head = [&](int i) { return hk * z.group + (begin + i) / per_head; };
-  auto tile = [&](int i) { return first + (begin + i) % per_head; };
-  // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
-  // share with others their rows of q and dout are cleared (by a whole warp), so that whatever they hold meets a probability of
-  // 0 as 0.
-  auto clear_blind = [&](int i, uint32_t at) {
-    const int blind = -off - tile(i) * kTile;
-    if (z.causal && blind > 0) zero_rows<D>(at, kTile * 128, 0, min(kTile, blind));
-    return true;
+  const int off = z.lk - z.lq, q_tiles = (z.lq + kTile - 1) / kTile;
+  struct Walk {
+    Item it;
+    int k0, n, first, per_head, begin, count;
   };
+  auto walk_of = [&](int id) {
+    Walk w;
+    w.it = item_of(p, id, z.kv_heads);
+    w.k0 = w.it.tile * kTile;
+    w.n = keys_of(z, w.it.b);
+    w.first = z.causal ? min(q_tiles, max(0, w.k0 - off) / kTile) : 0;         // the first query tile with a row that sees a key here
+    w.per_head = w.k0 < w.n ? q_tiles - w.first : 0;
+    w.begin = w.it.split * p.per_split;
+    w.count = max(0, min(z.group * w.per_head, w.begin + p.per_split) - w.begin);
+    return w;
+  };
+  // pass i of a walk: query tile `tile_at` of head `head_at`
+  auto head_at = [&](const Walk& w, int i) { return w.it.head * z.group + (w.begin + i) / w.per_head; };
+  auto tile_at = [&](const Walk& w, int i) { return w.first + (w.begin + i) % w.per_head; };
   auto g_at = [](int i) { return i % C::kG; };
   auto q_at = [](int i) { return C::kG + i % C::kQ; };
+  // r counts the CTA's passes, x its items with any, bits holds the phases of the stages; each role for itself
+  int r = 0, x = 0;
+  uint32_t bits = 0;
 
   if (warp == kTmaWarp) {
-    // ------------------------------------------------------------ TMA producer: q0, dout0 (with lse2, delta), q1, ...
-    if (lane == 0 && count > 0) {
+    // ------------------------------------------------------------ TMA producer: K, V, then q0, dout0 (with lse2, delta), q1, ...
+    bool ok = lane == 0;
+    bits = ~0u;                            // of the stages' release: all are free at first
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+      const Walk w = walk_of(id);
+      if (w.count == 0) continue;
+      ok = x == 0 || mbar_wait(m.bar(kFixedFree), (x - 1) & 1, &abort_flag);
+      if (!ok) break;
       mbar_expect_tx(m.bar(kFixedFull), 2 * C::kBytes);
-      load_rows<D, kTile>(m.fixed(0), &map_k, m.bar(kFixedFull), k0, hk, b);
-      load_rows<D, kTile>(m.fixed(1), &map_v, m.bar(kFixedFull), k0, hk, b);
-      for (int i = 0; i < count; ++i) {
-        const int s = q_at(i), r = g_at(i), h = head(i), q0 = tile(i) * kTile;
-        if (!mbar_wait(m.empty(s), ((i / C::kQ) & 1) ^ 1, &abort_flag)) break;
+      load_rows<D, kTile>(m.fixed(0), &map_k, m.bar(kFixedFull), w.k0, w.it.head, w.it.b);
+      load_rows<D, kTile>(m.fixed(1), &map_v, m.bar(kFixedFull), w.k0, w.it.head, w.it.b);
+      for (int i = 0; i < w.count && ok; ++i) {
+        const int s = q_at(i), g = g_at(i), h = head_at(w, i), q0 = tile_at(w, i) * kTile;
+        ok = mbar_wait(m.empty(s), phase_of(bits, s), &abort_flag);
+        if (!ok) break;
         mbar_expect_tx(m.full(s), C::kBytes);
-        load_rows<D, kTile>(m.stage(s), &map_q, m.full(s), q0, h, b);
-        if (!mbar_wait(m.empty(r), ((i / C::kG) & 1) ^ 1, &abort_flag)) break;
-        mbar_expect_tx(m.full(r), C::kBytes + C::kRowBytes);
-        const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + q0;
-        bulk_load(m.row_data(r), p.lse2 + at, kTile * 4, m.full(r));
-        bulk_load(m.row_data(r) + kTile * 4, p.delta + at, kTile * 4, m.full(r));
-        load_rows<D, kTile>(m.stage(r), &map_do, m.full(r), q0, h, b);
+        load_rows<D, kTile>(m.stage(s), &map_q, m.full(s), q0, h, w.it.b);
+        ok = mbar_wait(m.empty(g), phase_of(bits, g), &abort_flag);
+        if (!ok) break;
+        mbar_expect_tx(m.full(g), C::kBytes + C::kRowBytes);
+        const int64_t at = (static_cast<int64_t>(w.it.b) * z.heads + h) * p.lq_pad + q0;
+        bulk_load(m.row_data(g), p.lse2 + at, kTile * 4, m.full(g));
+        bulk_load(m.row_data(g) + kTile * 4, p.delta + at, kTile * 4, m.full(g));
+        load_rows<D, kTile>(m.stage(g), &map_do, m.full(g), q0, h, w.it.b);
       }
+      ++x;
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
-    auto scores = [&](int i) {             // S^T(i) = K Q^T
-      if (!warp_wait(m.full(q_at(i)), (i / C::kQ) & 1, &abort_flag) || !clear_blind(i, m.stage(q_at(i)))) return false;
-      tc_fence_after();
-      product_ss<D>(tmem + C::kS, m.fixed(0), m.stage(q_at(i)));
-      tc_commit_warp(m.bar(kSFull));
-      return true;
-    };
-    auto gradients = [&](int i) {          // dP^T(i) = V dO^T
-      if (!warp_wait(m.full(g_at(i)), (i / C::kG) & 1, &abort_flag) || !clear_blind(i, m.stage(g_at(i)))) return false;
-      tc_fence_after();
-      product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage(g_at(i)));
-      tc_commit_warp(m.bar(kDpFull));
-      return true;
-    };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0);
-    for (int i = 0; i < count && ok; ++i) {
-      const bool more = i + 1 < count;
-      ok = warp_wait(m.bar(kPReady), i & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      product_ts<D>(tmem + C::kAcc0, tmem + C::kS, m.stage(g_at(i)), kTile / 16, i > 0);
-      ok = !more || scores(i + 1);
-      ok = ok && warp_wait(m.bar(kDsReady), i & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      tc_commit_warp(m.empty(g_at(i)));    // dV(i) and dP(i) are through with it, and delta has been read
-      product_ts<D>(tmem + C::kAcc1, tmem + C::kDp, m.stage(q_at(i)), kTile / 16, i > 0);
-      tc_commit_warp(m.empty(q_at(i)));
-      ok = !more || gradients(i + 1);
-    }
-    if (ok && count > 0) tc_commit_warp(m.bar(kDone));
-  } else {
-    // ------------------------------------------------------------ probabilities: thread = key, warpgroup w has 32 queries
-    const int w = warp >> 2, row = k0 + (threadIdx.x & 127);
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + C::kS + w * 32, dp_at = tmem + lanes + C::kDp + w * 32;
-    const bool row_ok = row < n;
     bool ok = true;
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+      const Walk w = walk_of(id);
+      if (w.count == 0) continue;
+      // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
+      // share with others their rows of q and dout are cleared (by a whole warp), so that whatever they hold meets a probability
+      // of 0 as 0.
+      auto clear_blind = [&](int i, uint32_t at) {
+        const int blind = -off - tile_at(w, i) * kTile;
+        if (z.causal && blind > 0) zero_rows<D>(at, kTile * 128, 0, min(kTile, blind));
+      };
+      auto scores = [&](int i) {           // S^T(i) = K Q^T
+        const int s = q_at(i);
+        if (!warp_wait(m.full(s), phase_of(bits, s), &abort_flag)) return false;
+        clear_blind(i, m.stage(s));
+        tc_fence_after();
+        product_ss<D>(tmem + C::kS, m.fixed(0), m.stage(s));
+        tc_commit_warp(m.bar(kSFull));
+        return true;
+      };
+      auto gradients = [&](int i) {        // dP^T(i) = V dO^T
+        const int g = g_at(i);
+        if (!warp_wait(m.full(g), phase_of(bits, g), &abort_flag)) return false;
+        clear_blind(i, m.stage(g));
+        tc_fence_after();
+        product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage(g));
+        tc_commit_warp(m.bar(kDpFull));
+        if (i + 1 == w.count) tc_commit_warp(m.bar(kFixedFree));
+        return true;
+      };
+      ok = warp_wait(m.bar(kFixedFull), x & 1, &abort_flag) && scores(0) && gradients(0);
+      for (int i = 0; i < w.count && ok; ++i) {
+        const bool more = i + 1 < w.count;
+        ok = warp_wait(m.bar(kPReady), (r + i) & 1, &abort_flag) &&
+             (i > 0 || x == 0 || warp_wait(m.bar(kAccFree), (x - 1) & 1, &abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        product_ts<D>(tmem + C::kAcc0, tmem + C::kS, m.stage(g_at(i)), kTile / 16, i > 0);
+        ok = (!more || scores(i + 1)) && warp_wait(m.bar(kDsReady), (r + i) & 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        tc_commit_warp(m.empty(g_at(i)));      // dV(i) and dP(i) are through with it, and delta has been read
+        product_ts<D>(tmem + C::kAcc1, tmem + C::kDp, m.stage(q_at(i)), kTile / 16, i > 0);
+        tc_commit_warp(m.empty(q_at(i)));
+        if (!more) tc_commit_warp(m.bar(kDone));
+        ok = !more || gradients(i + 1);
+      }
+      r += w.count;
+      ++x;
+    }
+  } else {
+    // ------------------------------------------------------------ probabilities: thread = key, warpgroup wg has 32 queries
+    const int wg = warp >> 2;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + C::kS + wg * 32, dp_at = tmem + lanes + C::kDp + wg * 32;
     const f2 c2 = f2_dup(p.c);
-    for (int i = 0; i < count; ++i) {
-      const uint32_t rows = m.row_data(g_at(i)) + w * 128;
-      // queries of these 32 before `from` do not see this key
-      int from = row_ok ? 0 : 32;
-      if (z.causal && row_ok) from = row - off - tile(i) * kTile - w * 32;
-      const bool edge = __any_sync(0xffffffffu, from > 0);
-      ok = warp_wait(m.full(g_at(i)), (i / C::kG) & 1, &abort_flag);
-      if (!ok) break;
-      f2 pr[16], rd[16];                 // what does not depend on a product is read while waiting for it
+    bool ok = true;
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+      const Walk w = walk_of(id);
+      const int row = w.k0 + (threadIdx.x & 127);
+      const bool row_ok = row < w.n;
+      for (int i = 0; i < w.count; ++i, ++r) {
+        const uint32_t rows = m.row_data(g_at(i)) + wg * 128;
+        // queries of these 32 before `from` do not see this key
+        int from = row_ok ? 0 : 32;
+        if (z.causal && row_ok) from = row - off - tile_at(w, i) * kTile - wg * 32;
+        const bool edge = __any_sync(0xffffffffu, from > 0);
+        ok = warp_wait(m.full(g_at(i)), phase_of(bits, g_at(i)), &abort_flag);
+        if (!ok) break;
+        f2 pr[16], rd[16];               // the log-sums are read while the scores are waited for (after it: 1310 instead of 950 cycles to P)
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) lds_pairs(rows + e * 8, rd[e], rd[e + 1]);
-      ok = warp_wait(m.bar(kSFull), i & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[32], word[16];
-      tc_ld32(s_at, s);
-      tc_wait_ld();
+        for (int e = 0; e < 16; e += 2) lds_pairs(rows + e * 8, rd[e], rd[e + 1]);
+        ok = warp_wait(m.bar(kSFull), r & 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[32], word[16];
+        tc_ld32(s_at, s);
+        tc_wait_ld();
 #pragma unroll
-      for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, rd[e]), e);
-      if (edge) {
+        for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, rd[e]), e);
+        if (edge) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pr[e] = f2_make(2 * e >= from ? f2_lo(pr[e]) : 0.f, 2 * e + 1 >= from ? f2_hi(pr[e]) : 0.f);
-      }
+          for (int e = 0; e < 16; ++e) pr[e] = f2_make(2 * e >= from ? f2_lo(pr[e]) : 0.f, 2 * e + 1 >= from ? f2_hi(pr[e]) : 0.f);
+        }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) word[e] = bf16_of_f2(pr[e]);
-      tc_st16(s_at, word);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kPReady));
+        for (int e = 0; e < 16; ++e) word[e] = bf16_of_f2(pr[e]);
+        tc_st16(s_at, word);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(m.bar(kPReady));
 
-      ok = warp_wait(m.bar(kDpFull), i & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      tc_ld32(dp_at, s);
-      tc_wait_ld();
+        ok = warp_wait(m.bar(kDpFull), r & 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        tc_ld32(dp_at, s);
+        tc_wait_ld();
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        f2 d0, d1;
-        lds_pairs(rows + kTile * 4 + e * 8, d0, d1);
-        word[e] = bf16_of_f2(f2_mul(pr[e], f2_add(pair_of(s, e), d0)));
-        word[e + 1] = bf16_of_f2(f2_mul(pr[e + 1], f2_add(pair_of(s, e + 1), d1)));
-      }
-      if (!row_ok) {                     // what lies behind the sample's keys may be NaN
+        for (int e = 0; e < 16; e += 2) {
+          f2 d0, d1;
+          lds_pairs(rows + kTile * 4 + e * 8, d0, d1);
+          word[e] = bf16_of_f2(f2_mul(pr[e], f2_add(pair_of(s, e), d0)));
+          word[e + 1] = bf16_of_f2(f2_mul(pr[e + 1], f2_add(pair_of(s, e + 1), d1)));
+        }
+        if (!row_ok) {                   // what lies behind the sample's keys may be NaN
 #pragma unroll
-        for (int e = 0; e < 16; ++e) word[e] = 0u;
+          for (int e = 0; e < 16; ++e) word[e] = 0u;
+        }
+        tc_st16(dp_at, word);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(m.bar(kDsReady));
       }
-      tc_st16(dp_at, word);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kDsReady));
+      if (ok && w.count > 0) {
+        ok = warp_wait(m.bar(kDone), x & 1, &abort_flag);
+        tc_fence_after();
+      }
+      // warpgroups 0 and 1: the halves of dV; 2 and 3: of dK
+      const int64_t at = ((static_cast<int64_t>(w.it.b) * z.lk + row) * z.kv_heads + w.it.head) * D + (wg & 1) * (D / 2);
+      __nv_bfloat16* dst = wg < 2 ? p.dv : p.dk;
+      float* part = wg < 2 ? p.part0 : p.part1;
+      store_row<D / 2>(tmem + lanes + (wg < 2 ? C::kAcc0 : C::kAcc1) + (wg & 1) * (D / 2), w.count > 0, wg < 2 ? 1.f : p.scale,
+                       ok && row < z.lk, dst ? dst + at : nullptr, part ? part + w.it.split * p.elements + at : nullptr);
+      if (w.count > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(m.bar(kAccFree));
+        ++x;
+      }
     }
-    if (ok && count > 0) {
-      ok = warp_wait(m.bar(kDone), 0, &abort_flag);
-      tc_fence_after();
-    }
-    // warpgroups 0 and 1: the halves of dV; 2 and 3: of dK
-    const int64_t at = ((static_cast<int64_t>(b) * z.lk + row) * z.kv_heads + hk) * D + (w & 1) * (D / 2);
-    __nv_bfloat16* dst = w < 2 ? p.dv : p.dk;
-    float* part = w < 2 ? p.part0 : p.part1;
-    store_row<D / 2>(tmem + lanes + (w < 2 ? C::kAcc0 : C::kAcc1) + (w & 1) * (D / 2), count > 0, w < 2 ? 1.f : p.scale, ok && row < z.lk,
-                     dst ? dst + at : nullptr, part ? part + split * p.elements + at : nullptr);
   }
   teardown(&abort_flag, p.status, tmem, warp);
 }
 
 // ------------------------------------------------------------------------------------------------ queries: dQ
-// grid (query tiles * splits, heads, batch). P stays in registers here, so the scores have two buffers and S(j + 1) is ready
+// P stays in registers here, so the scores have two buffers and S(j + 1) is ready
 // when the warpgroups come to it.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -382,102 +448,146 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
   constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
 
   const Sizes& z = p.z;
-  const int split = blockIdx.x % p.splits, qt = blockIdx.x / p.splits, h = blockIdx.y, b = blockIdx.z;
-  const int hk = h / z.group, q0 = qt * kTile, n = keys_of(z, b);
-  const int lim_tile = key_limit(z, n, min(z.lq, q0 + kTile) - 1);
-  const int j0 = split * p.per_split, count = max(0, min((lim_tile + kTile - 1) / kTile, j0 + p.per_split) - j0);
+  struct Walk {
+    Item it;
+    int q0, n, j0, count;
+  };
+  auto walk_of = [&](int id) {
+    Walk w;
+    w.it = item_of(p, id, z.heads);
+    w.q0 = w.it.tile * kTile;
+    w.n = keys_of(z, w.it.b);
+    w.j0 = w.it.split * p.per_split;
+    const int lim = key_limit(z, w.n, min(z.lq, w.q0 + kTile) - 1);
+    w.count = max(0, min((lim + kTile - 1) / kTile, w.j0 + p.per_split) - w.j0);
+    return w;
+  };
+  // r counts the CTA's passes, x its items with any, bits holds the phases of the stages (of the score buffers); each role for itself
+  int r = 0, x = 0;
+  uint32_t bits = 0;
 
   if (warp == kTmaWarp) {
-    // ------------------------------------------------------------ TMA producer: K0, V0, K1, V1, ...
-    if (lane == 0 && count > 0) {
+    // ------------------------------------------------------------ TMA producer: q, dout, then K0, V0, K1, V1, ...
+    bool ok = lane == 0;
+    bits = ~0u;                            // of the stages' release: all are free at first
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+      const Walk w = walk_of(id);
+      if (w.count == 0) continue;
+      ok = x == 0 || mbar_wait(m.bar(kFixedFree), (x - 1) & 1, &abort_flag);
+      if (!ok) break;
       mbar_expect_tx(m.bar(kFixedFull), 2 * C::kBytes);
-      load_rows<D, kTile>(m.fixed(0), &map_q, m.bar(kFixedFull), q0, h, b);
-      load_rows<D, kTile>(m.fixed(1), &map_do, m.bar(kFixedFull), q0, h, b);
-      for (int i = 0; i < 2 * count; ++i) {
+      load_rows<D, kTile>(m.fixed(0), &map_q, m.bar(kFixedFull), w.q0, w.it.head, w.it.b);
+      load_rows<D, kTile>(m.fixed(1), &map_do, m.bar(kFixedFull), w.q0, w.it.head, w.it.b);
+      for (int i = 0; i < 2 * w.count; ++i) {
         const int s = i % C::kStages;
-        if (!mbar_wait(m.empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
+        ok = mbar_wait(m.empty(s), phase_of(bits, s), &abort_flag);
+        if (!ok) break;
         mbar_expect_tx(m.full(s), C::kBytes);
-        load_rows<D, kTile>(m.stage(s), (i & 1) ? &map_v : &map_k, m.full(s), (j0 + (i >> 1)) * kTile, hk, b);
+        load_rows<D, kTile>(m.stage(s), (i & 1) ? &map_v : &map_k, m.full(s), (w.j0 + (i >> 1)) * kTile, w.it.head / z.group, w.it.b);
       }
+      ++x;
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
-    auto wait_stage = [&](int i) { return warp_wait(m.full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
-    auto scores = [&](int j) {             // S(j) = Q K_j^T; the keys' rows behind the sample's length are cleared for dS K
-      const int s = 2 * j % C::kStages, keys = min(kTile, n - (j0 + j) * kTile);
-      if (!wait_stage(2 * j)) return false;
-      if (keys & 15) zero_rows<D>(m.stage(s), kTile * 128, keys, (keys + 15) & ~15);
-      tc_fence_after();
-      product_ss<D>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(s));
-      tc_commit_warp(m.bar(kSFull + (j & 1)));
-      return true;
-    };
-    auto gradients = [&](int j) {          // dP(j) = dO V_j^T
-      if (!wait_stage(2 * j + 1)) return false;
-      tc_fence_after();
-      product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage((2 * j + 1) % C::kStages));
-      tc_commit_warp(m.bar(kDpFull));
-      tc_commit_warp(m.empty((2 * j + 1) % C::kStages));
-      return true;
-    };
-    bool ok = count > 0 && warp_wait(m.bar(kFixedFull), 0, &abort_flag) && scores(0) && gradients(0) && (count == 1 || scores(1));
-    for (int j = 0; j < count && ok; ++j) {          // dS(j) is ready: dQ += dS K, the next dP, the scores after the next
-      ok = warp_wait(m.bar(kDsReady), j & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      product_ts<D>(tmem + C::kAcc0, tmem + C::kDp, m.stage(2 * j % C::kStages), (min(kTile, n - (j0 + j) * kTile) + 15) / 16, j > 0);
-      tc_commit_warp(m.empty(2 * j % C::kStages));
-      ok = (j + 1 >= count || gradients(j + 1)) && (j + 2 >= count || scores(j + 2));
+    bool ok = true;
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+      const Walk w = walk_of(id);
+      if (w.count == 0) continue;
+      auto k_stage = [&](int j) { return 2 * j % C::kStages; };
+      auto v_stage = [&](int j) { return (2 * j + 1) % C::kStages; };
+      auto keys_in = [&](int j) { return min(kTile, w.n - (w.j0 + j) * kTile); };
+      auto scores = [&](int j) {           // S(j) = Q K_j^T; the keys' rows behind the sample's length are cleared for dS K
+        const int s = k_stage(j), keys = keys_in(j);
+        if (!warp_wait(m.full(s), phase_of(bits, s), &abort_flag)) return false;
+        if (keys & 15) zero_rows<D>(m.stage(s), kTile * 128, keys, (keys + 15) & ~15);
+        tc_fence_after();
+        product_ss<D>(tmem + ((j & 1) ? kS1 : C::kS), m.fixed(0), m.stage(s));
+        tc_commit_warp(m.bar(kSFull + (j & 1)));
+        return true;
+      };
+      auto gradients = [&](int j) {        // dP(j) = dO V_j^T
+        const int s = v_stage(j);
+        if (!warp_wait(m.full(s), phase_of(bits, s), &abort_flag)) return false;
+        tc_fence_after();
+        product_ss<D>(tmem + C::kDp, m.fixed(1), m.stage(s));
+        tc_commit_warp(m.bar(kDpFull));
+        tc_commit_warp(m.empty(s));
+        if (j + 1 == w.count) tc_commit_warp(m.bar(kFixedFree));      // S(j) came before
+        return true;
+      };
+      ok = warp_wait(m.bar(kFixedFull), x & 1, &abort_flag) && scores(0) && (w.count == 1 || scores(1)) && gradients(0);
+      for (int j = 0; j < w.count && ok; ++j) {      // dS(j) is ready: dQ += dS K, the next dP, the scores after the next
+        ok = warp_wait(m.bar(kDsReady), (r + j) & 1, &abort_flag) &&
+             (j > 0 || x == 0 || warp_wait(m.bar(kAccFree), (x - 1) & 1, &abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        product_ts<D>(tmem + C::kAcc0, tmem + C::kDp, m.stage(k_stage(j)), (keys_in(j) + 15) / 16, j > 0);
+        tc_commit_warp(m.empty(k_stage(j)));
+        if (j + 1 == w.count) tc_commit_warp(m.bar(kDone));
+        ok = (j + 1 >= w.count || gradients(j + 1)) && (j + 2 >= w.count || scores(j + 2));
+      }
+      r += w.count;
+      ++x;
     }
-    if (ok && count > 0) tc_commit_warp(m.bar(kDone));
   } else {
-    // ------------------------------------------------------------ probabilities: thread = query, warpgroup w has 32 keys
-    const int w = warp >> 2, row = q0 + (threadIdx.x & 127), col = w * 32;
+    // ------------------------------------------------------------ probabilities: thread = query, warpgroup wg has 32 keys
+    const int wg = warp >> 2, col = wg * 32;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t dp_at = tmem + lanes + C::kDp + col;
-    const int lim = key_limit(z, n, row);
-    const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
-    const int64_t r = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + row;
-    const f2 c2 = f2_dup(p.c), lse = f2_dup(p.lse2[r]), delta = f2_dup(p.delta[r]);
+    const f2 c2 = f2_dup(p.c);
     bool ok = true;
-    for (int j = 0; j < count; ++j) {
-      ok = warp_wait(m.bar(kSFull + (j & 1)), (j >> 1) & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[32], word[16];
-      tc_ld32(tmem + lanes + ((j & 1) ? kS1 : C::kS) + col, s);
-      tc_wait_ld();
-      f2 pr[16];
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+      const Walk w = walk_of(id);
+      const int row = w.q0 + (threadIdx.x & 127), h = w.it.head, b = w.it.b;
+      const int lim = key_limit(z, w.n, row);
+      const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
+      const int64_t at = (static_cast<int64_t>(b) * z.heads + h) * p.lq_pad + row;
+      const f2 lse = f2_dup(p.lse2[at]), delta = f2_dup(p.delta[at]);
+      for (int j = 0; j < w.count; ++j, ++r) {
+        ok = warp_wait(m.bar(kSFull + (j & 1)), phase_of(bits, j & 1), &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[32], word[16];
+        tc_ld32(tmem + lanes + ((j & 1) ? kS1 : C::kS) + col, s);
+        tc_wait_ld();
+        f2 pr[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, lse), e);
-      ok = warp_wait(m.bar(kDpFull), j & 1, &abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      tc_ld32(dp_at, s);
-      tc_wait_ld();
-      const int from = lim - (j0 + j) * kTile - col;         // keys from here on are not seen
+        for (int e = 0; e < 16; ++e) pr[e] = exp2_mixed(f2_fma(pair_of(s, e), c2, lse), e);
+        ok = warp_wait(m.bar(kDpFull), r & 1, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        tc_ld32(dp_at, s);
+        tc_wait_ld();
+        const int key = (w.j0 + j) * kTile + col, from = lim - key;      // keys from here on are not seen
 #pragma unroll
-      for (int e = 0; e < 16; ++e) pr[e] = f2_mul(pr[e], f2_add(pair_of(s, e), delta));
-      if ((j0 + j) * kTile + col + 32 > lim_all) {           // what lies behind the sample's keys may be NaN
+        for (int e = 0; e < 16; ++e) pr[e] = f2_mul(pr[e], f2_add(pair_of(s, e), delta));
+        if (key + 32 > lim_all) {        // what lies behind the sample's keys may be NaN
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pr[e] = f2_make(2 * e < from ? f2_lo(pr[e]) : 0.f, 2 * e + 1 < from ? f2_hi(pr[e]) : 0.f);
+          for (int e = 0; e < 16; ++e) pr[e] = f2_make(2 * e < from ? f2_lo(pr[e]) : 0.f, 2 * e + 1 < from ? f2_hi(pr[e]) : 0.f);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) word[e] = bf16_of_f2(pr[e]);
+        tc_st16(dp_at, word);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(m.bar(kDsReady));
       }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) word[e] = bf16_of_f2(pr[e]);
-      tc_st16(dp_at, word);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(m.bar(kDsReady));
+      if (ok && w.count > 0) {
+        ok = warp_wait(m.bar(kDone), x & 1, &abort_flag);
+        tc_fence_after();
+      }
+      const int64_t dense = ((static_cast<int64_t>(b) * z.heads + h) * z.lq + row) * D + wg * (D / 4);
+      store_row<D / 4>(tmem + lanes + C::kAcc0 + wg * (D / 4), w.count > 0, p.scale, ok && row < z.lq,
+                       p.dq + b * p.sdq.b + row * p.sdq.l + h * p.sdq.h + wg * (D / 4),
+                       p.part0 ? p.part0 + w.it.split * p.elements + dense : nullptr);
+      if (w.count > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(m.bar(kAccFree));
+        ++x;
+      }
     }
-    if (ok && count > 0) {
-      ok = warp_wait(m.bar(kDone), 0, &abort_flag);
-      tc_fence_after();
-    }
-    const int64_t dense = ((static_cast<int64_t>(b) * z.heads + h) * z.lq + row) * D + w * (D / 4);
-    store_row<D / 4>(tmem + lanes + C::kAcc0 + w * (D / 4), count > 0, p.scale, ok && row < z.lq,
-                     p.dq + b * p.sdq.b + row * p.sdq.l + h * p.sdq.h + w * (D / 4),
-                     p.part0 ? p.part0 + split * p.elements + dense : nullptr);
   }
   teardown(&abort_flag, p.status, tmem, warp);
 }
@@ -522,7 +632,7 @@ int split_count(int64_t ctas, int64_t items) {
 struct Plan {
   int64_t lq_pad, row_floats;            // lse2 and delta
   int key_splits, key_per, query_splits, query_per;
-  int64_t key_elements, query_elements;
+  int64_t key_elements, query_elements, key_items, query_items;
   Plan(const Shape& s, bool want_keys, bool want_queries) {
     const int64_t q_tiles = ceil_div(s.lq, kTile), k_tiles = ceil_div(s.lk, kTile), group = s.heads / s.kv_heads;
     lq_pad = q_tiles * kTile;
@@ -533,6 +643,8 @@ struct Plan {
     query_per = static_cast<int>(std::max<int64_t>(1, ceil_div(k_tiles, query_splits)));
     key_elements = s.batch * s.lk * s.kv_heads * s.d;
     query_elements = s.batch * s.lq * s.heads * s.d;
+    key_items = k_tiles * key_splits * s.kv_heads * s.batch;
+    query_items = q_tiles * query_splits * s.heads * s.batch;
   }
   // the partial sums of the keys are read before those of the queries are written: one buffer
   int64_t part_floats() const {
@@ -552,6 +664,10 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
   ANIMA_REQUIRE(rc == cudaSuccess, ANIMA_E_CUDA, "%s: cannot reserve %d bytes of shared memory: %s", who, C::kSmem,
                 cudaGetErrorString(rc));
   float* part = p.part0;
+  // One CTA a SM goes through all its items; causal, whose items differ in length, four rounds of CTAs, which the GPU hands out
+  // as SMs get free ([4, 2047, 16 / 4 heads, 64] 293 -> 270 us; not causal, four rounds cost [8, 4096 x 512] 597 -> 614).
+  const int64_t most = (p.z.causal ? 4LL : 1LL) * sm_count();
+  auto grid = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min(items, most))); };
   if (rows.rows) {
     launch_after(attention_rows_kernel<D>, dim3(static_cast<unsigned>(ceil_div(rows.rows, 256 / (D / 8)))), dim3(256), 0, st, rows);
     ANIMA_CHECK_LAUNCH(who);
@@ -568,8 +684,9 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
     p.elements = plan.key_elements;
     p.part0 = p.splits > 1 ? part : nullptr;
     p.part1 = p.splits > 1 ? part + p.splits * p.elements : nullptr;
-    const dim3 grid(static_cast<unsigned>(ceil_div(s.lk, kTile) * p.splits), static_cast<unsigned>(s.kv_heads), static_cast<unsigned>(s.batch));
-    launch_after(attention_bwd_keys_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
+    p.tiles = static_cast<int>(ceil_div(s.lk, kTile));
+    p.items = static_cast<int>(plan.key_items);
+    launch_after(attention_bwd_keys_kernel<D>, grid(p.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
     ANIMA_CHECK_LAUNCH(who);
     if (p.splits > 1) {
       if (p.dv)
@@ -583,8 +700,9 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
     p.per_split = plan.query_per;
     p.elements = plan.query_elements;
     p.part0 = p.splits > 1 ? part : nullptr;
-    const dim3 grid(static_cast<unsigned>(ceil_div(s.lq, kTile) * p.splits), static_cast<unsigned>(s.heads), static_cast<unsigned>(s.batch));
-    launch_after(attention_bwd_queries_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
+    p.tiles = static_cast<int>(ceil_div(s.lq, kTile));
+    p.items = static_cast<int>(plan.query_items);
+    launch_after(attention_bwd_queries_kernel<D>, grid(p.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
     ANIMA_CHECK_LAUNCH(who);
     if (p.splits > 1) return join(p.part0, p.dq, p.splits, p.elements, p.z.lq);
   }
@@ -600,7 +718,9 @@ using namespace anima;
 extern "C" int64_t anima_attention_bwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
                                                        int64_t head_dim, int causal) {
   if (int rc = attn::check_sizes("attention_bwd", batch, lq, lk, heads, kv_heads, head_dim)) return rc;
-  return attn::Plan(attn::Shape(batch, lq, lk, heads, kv_heads, head_dim, causal), true, true).bytes();
+  const attn::Plan plan(attn::Shape(batch, lq, lk, heads, kv_heads, head_dim, causal), true, true);
+  ANIMA_REQUIRE(plan.key_items < (1ll << 30) && plan.query_items < (1ll << 30), ANIMA_E_TOO_LARGE, "attention_bwd: too many tiles");
+  return plan.bytes();
 }
 
 extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides, const void* q, const int64_t* q_strides,

@@ -155,10 +155,10 @@ inline bool bind_context() {
   return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
-// Tensor map of a (batch, token, head, D) bf16 tensor, boxes of 128 tokens x 64 elements. A tensor without elements gets the
+// Tensor map of a (batch, token, head, D) bf16 tensor, boxes of `rows` tokens x 64 elements. A tensor without elements gets the
 // map of one that is never read (`stand_in`: any valid address).
 inline bool encode_heads(CUtensorMap* map, const void* p, const Strided& s, int64_t batch, int64_t len, int64_t heads, int64_t d,
-                         const void* stand_in) {
+                         const void* stand_in, uint32_t rows = kTile) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   const bool none = batch * len == 0;
@@ -166,7 +166,7 @@ inline bool encode_heads(CUtensorMap* map, const void* p, const Strided& s, int6
   // the stride of a dimension of one element is not used; any valid one will do
   auto bytes = [&](int64_t n, int64_t stride) { return (cuuint64_t)(n > 1 && !none ? stride * 2 : 2 * d); };
   const cuuint64_t strides[3] = {bytes(len, s.l), bytes(heads, s.h), bytes(batch, s.b)};
-  const cuuint32_t box[4] = {64, kTile, 1, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, rows, 1, 1}, step[4] = {1, 1, 1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(none ? stand_in : p), dims, strides, box, step,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

@@ -1,15 +1,20 @@
 // Attention, forward (formulas: attention_common.cuh): one pass over the keys with each row's running maximum and sum.
 //
-// A CTA owns two tiles of 128 queries of one head and walks the keys, 64 at a time. Per query tile and step
+// A CTA owns a tile of 128 queries of one head and walks the keys, 64 at a time. Per step
 //   S = Q K^T     tcgen05, both operands in shared memory, fp32 scores in tensor memory (lane = query, column = key);
-//   softmax       one warpgroup a query tile, one thread a row: 64 scores into registers, row maximum without shuffles,
+//   softmax       one warpgroup, one thread a row: 64 scores into registers, row maximum without shuffles,
 //                 p = 2^(s scale log2 e - m), rounded to bf16 for the second product (the sum takes the unrounded values), written
 //                 over the scores;
 //   O += P V      tcgen05 with P read from tensor memory, V as it lies (keys along rows: the MN-major form), fp32.
-// The scores of a query tile have two buffers: S of the step after next is issued behind O += P V, which frees its buffer, so
-// a warpgroup finds its next scores ready and the special-function unit, shared by both, never waits for the tensor cores.
-// A warp for each query tile issues its products (the waits of one overlap the products of the other), one feeds tiles of 128
-// keys of K and V through a ring of TMA boxes.
+// The scores have two buffers: S of the step after next is issued behind O += P V, which frees its buffer, so the warpgroup
+// finds its next scores ready. One warp issues the products, one feeds K and V through a ring of TMA boxes of 64 keys.
+// Two CTAs share an SM (half of its tensor memory and shared memory each): the maxima, sums, loads and waits of one fill the
+// special-function unit's and the tensor cores' pauses of the other, and so do a CTA's set-up, first loads and way out, 6000
+// cycles or four steps. One CTA with two query tiles reads K and V half as often, but was slower nearly everywhere
+// ([8, 4096 x 512, 16, 128] 224 against 206 us, [8, 4096 x 1024] 275 / 261, [2, 4096 x 4096] 245 / 240, [8, 4096 x 4096] 869 / 884,
+// [4, 4096 x 4096, 16, 64] 396 / 363).
+// O leaves through the query tile's shared memory and TMA stores (each thread holds a row: its own 16-byte stores took 3000
+// cycles a tile).
 // The running maximum of a row is only raised once a score exceeds it by 2^8: until then p is at most 256, which costs neither
 // bf16 (relative) nor the fp32 sums anything, and O, which lies in tensor memory, need not be rescaled.
 // Few rows (one token, a short text) leave SMs idle: the keys are then cut into ranges, whose normalised fp32 outputs and
@@ -23,20 +28,20 @@ namespace anima {
 namespace attn {
 namespace {
 
-constexpr int kThreads = 352;            // two softmax warpgroups, an MMA warp for each query tile, one TMA warp
-constexpr int kMmaWarp = 8, kTmaWarp = 10;
 constexpr int kStep = 64;                // keys of a step
 constexpr float kMaxSlack = 8.f;         // log2 of how far a score may exceed the maximum in use
 constexpr int kPoly = 1;                 // of four pairs of exponentials, those made on the multiply-add pipes
 
 template <int D>
 struct FwdCfg {
+  static constexpr int kMmaWarp = 4, kTmaWarp = 5, kThreads = 192;
+  static constexpr uint32_t kBytes = tile_bytes<D>(), kStepBytes = kBytes / 2;
   static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kBars = 2 * kStages + 14;
-  static constexpr int kSmem = (2 + kStages) * static_cast<int>(tile_bytes<D>()) + kBars * 8;
-  static_assert(kSmem <= 227 * 1024 - 16, "shared memory");
-  // tensor-memory columns: scores of tile t, buffer x at 128 t + 64 x
-  static constexpr uint32_t kS = 0, kO = 256;
+  static constexpr int kBars = 2 * kStages + 7;
+  static constexpr int kSmem = static_cast<int>(kBytes + kStages * kStepBytes) + kBars * 8 + 24;
+  static_assert(2 * (kSmem + 1024) <= 228 * 1024, "shared memory of two CTAs");
+  // tensor-memory columns: scores of buffer x at 64 x
+  static constexpr uint32_t kS = 0, kO = kTile, kCols = 256;
 };
 
 struct FwdParams {
@@ -52,142 +57,131 @@ struct FwdParams {
   int32_t* status;
 };
 
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
 // grid (q_blocks * splits, heads, batch)
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(FwdCfg<D>::kThreads, 2)
 attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FwdParams p) {
+                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o,
+                     const __grid_constant__ FwdParams p) {
   using C = FwdCfg<D>;
-  constexpr uint32_t kBytes = tile_bytes<D>();
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ volatile int abort_flag;
-  __shared__ uint32_t tmem_slot;
   const uint32_t base = smem_u32(smem);
-  auto q_smem = [&](int t) { return base + t * kBytes; };
-  auto kv_smem = [&](int s) { return base + (2 + s) * kBytes; };
-  const uint32_t bars = base + (2 + C::kStages) * kBytes;
+  const uint32_t q_smem = base;
+  auto kv_smem = [&](int s) { return base + C::kBytes + s * C::kStepBytes; };
+  const uint32_t bars = base + C::kBytes + C::kStages * C::kStepBytes;
   auto full = [&](int s) { return bars + 8 * s; };
   auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
   const uint32_t q_full = bars + 8 * (2 * C::kStages);
-  auto s_full = [&](int t, int x) { return q_full + 8 * (1 + 2 * t + x); };
-  auto p_full = [&](int t, int x) { return q_full + 8 * (5 + 2 * t + x); };
-  auto o_done = [&](int t, int x) { return q_full + 8 * (9 + 2 * t + x); };
-  const uint32_t first_done = q_full + 8 * 13;     // tile 0 is through its first softmax
+  auto s_full = [&](int x) { return q_full + 8 * (1 + x); };
+  auto o_done = [&](int x) { return q_full + 8 * (3 + x); };
+  auto p_full = [&](int x) { return q_full + 8 * (5 + x); };
+  volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (bars - base) + C::kBars * 8 + 8);
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (bars - base) + C::kBars * 8 + 16);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int i = 0; i < C::kBars; ++i) {
-      const bool p = i >= 2 * C::kStages + 5 && i < 2 * C::kStages + 9, e = i >= C::kStages && i < 2 * C::kStages;
-      mbar_init(bars + 8 * i, p ? 4 : (e ? 2 : 1));
-    }
+    for (int i = 0; i < C::kBars; ++i) mbar_init(bars + 8 * i, i >= 2 * C::kStages + 5 ? 4 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_o) : "memory");
   }
-  if (warp == kMmaWarp) tc_alloc(smem_u32(&tmem_slot), 512);
+  if (warp == C::kMmaWarp) tc_alloc(smem_u32(&tmem_slot), C::kCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   after_previous();
-  constexpr uint32_t tmem = 0;             // the address of an allocation of all 512 columns
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
   const Sizes& z = p.z;
   const int split = blockIdx.x / p.q_blocks, qb = blockIdx.x - split * p.q_blocks, h = blockIdx.y, b = blockIdx.z;
   const int hk = h / z.group;
-  const int q0 = qb * 2 * kTile;
+  const int q0 = qb * kTile;
   const int n = keys_of(z, b);
-  // this CTA's keys start at k0; query tile t takes count[t] steps
+  // this CTA's keys start at k0, in `count` steps
   const int j0 = split * p.tiles_per_split, k0 = j0 * kTile;
-  int count[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int first = q0 + t * kTile;
-    const int last = min(z.lq, first + kTile) - 1;
-    const int lim = first < z.lq ? min(key_limit(z, n, last), k0 + p.tiles_per_split * kTile) : 0;
-    count[t] = max(0, lim - k0 + kStep - 1) / kStep;
-  }
-  const int most = max(count[0], count[1]);
+  const int lim_tile = min(key_limit(z, n, min(z.lq, q0 + kTile) - 1), k0 + p.tiles_per_split * kTile);
+  const int count = max(0, lim_tile - k0 + kStep - 1) / kStep;
+  // the order of the ring: K0, K1, V0, K2, V1, ...
+  auto k_at = [](int u) { return u == 0 ? 0 : 2 * u - 1; };
+  auto v_at = [&](int u) { return 2 * u + (u + 1 < count ? 2 : 1); };
 
-  if (warp == kTmaWarp) {
-    // ------------------------------------------------------------ TMA producer: K0, V0, K1, V1, ...
-    if (lane == 0 && most > 0) {
-      mbar_expect_tx(q_full, kBytes * (count[1] > 0 ? 2 : 1));
-      load_rows<D, kTile>(q_smem(0), &map_q, q_full, q0, h, b);
-      if (count[1] > 0) load_rows<D, kTile>(q_smem(1), &map_q, q_full, q0 + kTile, h, b);
-      for (int i = 0; i < 2 * ((most + 1) / 2); ++i) {
+  if (warp == C::kTmaWarp) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0 && count > 0) {
+      mbar_expect_tx(q_full, C::kBytes);
+      load_rows<D, kTile>(q_smem, &map_q, q_full, q0, h, b);
+      for (int i = 0; i < 2 * count; ++i) {
         const int s = i % C::kStages;
+        const bool value = i == 2 * count - 1 || (i > 0 && !(i & 1));
+        const int u = value ? (i - 1) / 2 : (i + 1) / 2;
         if (!mbar_wait(empty(s), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
-        mbar_expect_tx(full(s), kBytes);
-        load_rows<D, kTile>(kv_smem(s), (i & 1) ? &map_v : &map_k, full(s), k0 + (i >> 1) * kTile, hk, b);
+        mbar_expect_tx(full(s), C::kStepBytes);
+        load_rows<D, kStep>(kv_smem(s), value ? &map_v : &map_k, full(s), k0 + u * kStep, hk, b);
       }
     }
-  } else if (warp >= kMmaWarp) {
-    // ------------------------------------------------------------ MMA issuer of query tile t
-    constexpr uint32_t kIdescS = tc_idesc_bf16(kTile, kStep), kIdescO = tc_idesc_bf16(kTile, D, true);
-    const int t = warp - kMmaWarp;
-    const uint64_t q_desc = tc_desc_sw128(q_smem(t));
+  } else if (warp == C::kMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint64_t q_desc = tc_desc_sw128(q_smem);
     auto arrived = [&](int i) { return warp_wait(full(i % C::kStages), (i / C::kStages) & 1, &abort_flag); };
     auto scores = [&](int u) {                 // S of step u
-      const uint64_t k = tc_desc_sw128(kv_smem((u >> 1) * 2 % C::kStages) + (u & 1) * (kStep * 128));
+      const int s = k_at(u) % C::kStages;
+      const uint64_t k = tc_desc_sw128(kv_smem(s));
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t at = (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2;   // 16 bytes a unit
-        tc_mma_ss(tmem + C::kS + t * kTile + (u & 1) * kStep, q_desc + at, k + at, kIdescS, i > 0);
-      }
-      tc_commit_warp(s_full(t, u & 1));
+      for (int i = 0; i < D / 16; ++i)         // 16 bytes a unit
+        tc_mma_ss(tmem + C::kS + (u & 1) * kStep, q_desc + (i >> 2) * (kTile * 128 / 16) + (i & 3) * 2,
+                  k + (i >> 2) * (kStep * 128 / 16) + (i & 3) * 2, tc_idesc_bf16(kTile, kStep), i > 0);
+      tc_commit_warp(s_full(u & 1));
+      tc_commit_warp(empty(s));
     };
-    // a stage is free when both tiles are through with it; a tile that takes no part in a step (causal, short) says so at once
-    bool ok = most > 0 && warp_wait(q_full, 0, &abort_flag) && arrived(0);
-    if (ok) {
+    bool ok = count > 0 && warp_wait(q_full, 0, &abort_flag);
+    for (int u = 0; u < min(2, count) && ok; ++u) {
+      ok = arrived(k_at(u));
       tc_fence_after();
-      // half a step apart: one tile's exponentials meet the other's maxima and sums
-      if (t == 1 && count[0] > 0) ok = warp_wait(first_done, 0, &abort_flag);
-      if (count[t] > 0) scores(0);
-      if (count[t] > 1) scores(1);
-      tc_commit_warp(empty(0));
+      if (ok) scores(u);
     }
-    for (int u = 0; u < most && ok; ++u) {
-      const int vi = (u >> 1) * 2 + 1, ki = vi + 1, vs = vi % C::kStages;
-      if (!(u & 1)) ok = arrived(vi) && (u + 2 >= most || arrived(ki));
+    for (int u = 0; u < count && ok; ++u) {
+      const int vs = v_at(u) % C::kStages;
+      const bool next = u + 2 < count;
+      // keys of the step that exist; the product over the others is left out, up to the next multiple of 16
+      const int keys = min(kStep, n - k0 - u * kStep), steps = (keys + 15) / 16;
+      ok = arrived(v_at(u)) && (!next || arrived(k_at(u + 2)));
       if (!ok) break;
-      if (u < count[t]) {
-        // keys of the step that exist; the product over the others is left out, up to the next multiple of 16
-        const int keys = min(kStep, n - k0 - u * kStep), steps = (keys + 15) / 16;
-        if (keys & 15) zero_rows<D>(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128, keys, steps * 16);   // by either warp: the same zeros
-        const uint64_t v = tc_desc_sw128(kv_smem(vs) + (u & 1) * (kStep * 128), kTile * 128);
-        ok = warp_wait(p_full(t, u & 1), (u >> 1) & 1, &abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        if (t == 0 && u == 0 && lane == 0) mbar_arrive(first_done);
-        const uint32_t o = tmem + C::kO + t * D, pr = tmem + C::kS + t * kTile + (u & 1) * kStep;
+      if (keys & 15) zero_rows<D>(kv_smem(vs), kStep * 128, keys, steps * 16);
+      const uint64_t v = tc_desc_sw128(kv_smem(vs), kStep * 128);
+      ok = warp_wait(p_full(u & 1), (u >> 1) & 1, &abort_flag);
+      if (!ok) break;
+      tc_fence_after();
 #pragma unroll
-        for (int i = 0; i < kStep / 16; ++i)
-          if (i < steps) tc_mma_ts(o, pr + i * 8, v + i * (16 * 128 / 16), kIdescO, u > 0 || i > 0);
-        tc_commit_warp(o_done(t, u & 1));
-        if (u + 2 < count[t]) scores(u + 2);
-      }
-      if (u & 1) {
-        tc_commit_warp(empty(vs));
-        if (u + 2 < most) tc_commit_warp(empty(ki % C::kStages));
-      }
+      for (int i = 0; i < kStep / 16; ++i)
+        if (i < steps)
+          tc_mma_ts(tmem + C::kO, tmem + C::kS + (u & 1) * kStep + i * 8, v + i * (16 * 128 / 16), tc_idesc_bf16(kTile, D, true), u > 0 || i > 0);
+      tc_commit_warp(o_done(u & 1));
+      tc_commit_warp(empty(vs));
+      if (next) scores(u + 2);
     }
   } else {
-    // ------------------------------------------------------------ softmax: warpgroup t, thread = row
-    const int t = warp >> 2;
-    const int row = q0 + t * kTile + (threadIdx.x & 127);
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + C::kS + t * kTile, o_at = tmem + lanes + C::kO + t * D;
+    // ------------------------------------------------------------ softmax: thread = row
+    const int row = q0 + threadIdx.x;
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t s_at = tmem + lanes + C::kS, o_at = tmem + lanes + C::kO;
     const int lim = key_limit(z, n, row);
     // the warp's first row sees the fewest keys: steps that end before that need no mask
     const int lim_all = __shfl_sync(0xffffffffu, lim, 0);
     float m = -INFINITY, used = 0.f;     // maximum in use (raw scores), m * c (0 while there is none)
     f2 sum[4] = {0ull, 0ull, 0ull, 0ull};
     bool ok = true;
-    for (int u = 0; u < count[t]; ++u) {
+    for (int u = 0; u < count; ++u) {
       const uint32_t at = s_at + (u & 1) * kStep;
-      ok = warp_wait(s_full(t, u & 1), (u >> 1) & 1, &abort_flag);
+      ok = warp_wait(s_full(u & 1), (u >> 1) & 1, &abort_flag);
       if (!ok) break;
       tc_fence_after();
       uint32_t s[2][32];
@@ -218,7 +212,7 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
           used = m * p.c;
         }
         if (u > 0) {                       // the product of the step before is the last one under way: S(u) came behind the others
-          ok = warp_wait(o_done(t, (u - 1) & 1), ((u - 1) >> 1) & 1, &abort_flag);
+          ok = warp_wait(o_done((u - 1) & 1), ((u - 1) >> 1) & 1, &abort_flag);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
@@ -248,14 +242,14 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(t, u & 1));
+      if (lane == 0) mbar_arrive(p_full(u & 1));
       // the row's sum, behind what the tensor cores wait for
 #pragma unroll
       for (int e = 0; e < 32; ++e) sum[e & 3] = f2_add(sum[e & 3], y[e]);
     }
     // ------------------------------------------------------------ epilogue
-    if (ok && count[t] > 0) {
-      ok = warp_wait(o_done(t, (count[t] - 1) & 1), ((count[t] - 1) >> 1) & 1, &abort_flag);
+    if (ok && count > 0) {
+      ok = warp_wait(o_done((count - 1) & 1), ((count - 1) >> 1) & 1, &abort_flag);
       tc_fence_after();
     }
     const float l = f2_sum(f2_add(f2_add(sum[0], sum[1]), f2_add(sum[2], sum[3])));
@@ -265,7 +259,7 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     const float total = l == 0.f ? -INFINITY : used + log2_approx(l);      // base 2
     if (p.part_o != nullptr) {
       if (live) p.part_lse[split * p.rows + at] = total;
-      if (count[t] > 0) {
+      if (count > 0) {
 #pragma unroll 1
         for (int i = 0; i < D / 32; ++i) {
           uint32_t o[32];
@@ -282,27 +276,41 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
       }
     } else {
       if (live && p.lse) p.lse[at] = total * kLn2;
-      __nv_bfloat16* dst = p.out + b * p.so.b + row * p.so.l + h * p.so.h;
-#pragma unroll 1
+      // through the query tile's memory, which no product reads any more, swizzled as TMA wants it; rows behind the last query
+      // are left out by the store
+      const int r = threadIdx.x;
+      const uint32_t to = q_smem + r * 128;
+#pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         uint32_t o[32];
         __syncwarp();
-        if (count[t] > 0) {
+        if (count > 0) {
           tc_ld32(o_at + i * 32, o);
           tc_wait_ld();
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0u;
         }
-        if (!live) continue;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float f[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[8 * e + x]) * inv;
-          *reinterpret_cast<uint4*>(dst + i * 32 + e * 8) = pack8(f);
+          const uint4 w = pack8(f);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                       ::"r"(to + (i >> 1) * (kTile * 128) + ((((i & 1) * 4 + e) ^ (r & 7)) << 4)), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                       : "memory");
         }
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      const int first = row - lane;              // of the warp's 32 rows
+      if (lane == 0 && ok && first < z.lq) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) tma_store_4d(&map_o, to + c * (kTile * 128), c * 64, first, h, b);
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+      __syncwarp();
     }
   }
 
@@ -314,9 +322,9 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == C::kMmaWarp) {
     tc_fence_after();
-    tc_dealloc(tmem, 512);
+    tc_dealloc(tmem, C::kCols);
   }
 }
 
@@ -352,15 +360,21 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
   if (p.lse && lane == 0) p.lse[at] = l == 0.f ? -INFINITY : (ref + log2_approx(l)) * kLn2;
 }
 
-// Ranges the keys are cut into: as many as give every SM two CTAs, none shorter than four tiles.
-int split_count(const Shape& s) {
-  const int64_t ctas = ceil_div(s.lq, 2 * kTile) * s.heads * s.batch, tiles = ceil_div(s.lk, kTile);
-  if (ctas == 0 || ctas >= sm_count()) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(2LL * sm_count(), ctas), tiles / 4)));
-}
+struct Plan {
+  int q_blocks, splits, tiles_per_split;
+  explicit Plan(const Shape& s) {
+    q_blocks = static_cast<int>(ceil_div(s.lq, kTile));
+    // Ranges the keys are cut into where there are fewer CTAs than SMs: as many as fill every SM once (more only add to what is
+    // joined: [8, 1 x 16384, 16 / 4 heads, 128] 43 us with twice as many, 35 so), none shorter than three tiles.
+    const int64_t ctas = q_blocks * s.heads * s.batch, key_tiles = ceil_div(s.lk, kTile);
+    splits = 1;
+    if (ctas > 0 && ctas < sm_count()) splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2LL * sm_count() / ctas, key_tiles / 3)));
+    tiles_per_split = static_cast<int>(ceil_div(std::max<int64_t>(1, key_tiles), splits));
+  }
+};
 
 template <int D>
-int launch(const char* who, const CUtensorMap* maps, FwdParams p, const Shape& s, cudaStream_t st) {
+int launch(const char* who, const CUtensorMap* maps, const FwdParams& p, const Shape& s, cudaStream_t st) {
   using C = FwdCfg<D>;
   static PerDeviceOnce once;
   const cudaError_t rc = per_device_once(once, [] {
@@ -369,7 +383,7 @@ int launch(const char* who, const CUtensorMap* maps, FwdParams p, const Shape& s
   ANIMA_REQUIRE(rc == cudaSuccess, ANIMA_E_CUDA, "%s: cannot reserve %d bytes of shared memory: %s", who, C::kSmem,
                 cudaGetErrorString(rc));
   const dim3 grid(static_cast<unsigned>(p.q_blocks * p.splits), static_cast<unsigned>(s.heads), static_cast<unsigned>(s.batch));
-  launch_after(attention_fwd_kernel<D>, grid, dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], p);
+  launch_after(attention_fwd_kernel<D>, grid, dim3(C::kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
   ANIMA_CHECK_LAUNCH(who);
   if (p.splits > 1) {
     launch_after(attention_join_kernel<D>, dim3(static_cast<unsigned>(ceil_div(p.rows, 8))), dim3(256), 0, st, p);
@@ -387,7 +401,7 @@ using namespace anima;
 extern "C" int64_t anima_attention_fwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
                                                        int64_t head_dim, int causal) {
   if (int rc = attn::check_sizes("attention_fwd", batch, lq, lk, heads, kv_heads, head_dim)) return rc;
-  const int64_t splits = attn::split_count(attn::Shape(batch, lq, lk, heads, kv_heads, head_dim, causal));
+  const int64_t splits = attn::Plan(attn::Shape(batch, lq, lk, heads, kv_heads, head_dim, causal)).splits;
   return splits > 1 ? splits * batch * heads * lq * (head_dim + 1) * 4 : 0;
 }
 
@@ -420,18 +434,20 @@ extern "C" int anima_attention_fwd(const void* q, const int64_t* q_strides, cons
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   p.status = status;
-  p.q_blocks = static_cast<int>(ceil_div(s.lq, 2 * attn::kTile));
-  p.splits = attn::split_count(s);
-  p.tiles_per_split = static_cast<int>(ceil_div(std::max<int64_t>(1, ceil_div(s.lk, attn::kTile)), p.splits));
+  const attn::Plan plan(s);
+  p.q_blocks = plan.q_blocks;
+  p.splits = plan.splits;
+  p.tiles_per_split = plan.tiles_per_split;
   p.rows = s.batch * s.heads * s.lq;
   if (p.splits > 1) {
     p.part_o = static_cast<float*>(workspace);
     p.part_lse = p.part_o + p.splits * p.rows * head_dim;
   }
-  CUtensorMap maps[3];
+  CUtensorMap maps[4];
   ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, q) &&
-                    attn::encode_heads(&maps[1], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, q) &&
-                    attn::encode_heads(&maps[2], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, q),
+                    attn::encode_heads(&maps[1], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, q, attn::kStep) &&
+                    attn::encode_heads(&maps[2], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, q, attn::kStep) &&
+                    attn::encode_heads(&maps[3], out, p.so, s.batch, s.lq, s.heads, s.d, q, 32),
                 ANIMA_E_CUDA, "%s: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand)", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return head_dim == 64 ? attn::launch<64>(who, maps, p, s, st) : attn::launch<128>(who, maps, p, s, st);
