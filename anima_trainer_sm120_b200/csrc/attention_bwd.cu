@@ -49,35 +49,49 @@ struct RowsParams {
   const float* lse;
   float *lse2, *delta;
   int lq, lq_pad, heads;
-  int64_t rows;                          // batch * lq_pad * heads
 };
 
-// D / 8 lanes a row, rows in the order of memory
+// D / 8 lanes a row; a CTA takes kRowsPerCta (token, head) rows of a sample in the order of memory, all loads first. grid (., batch).
+constexpr int kRowsPerThread = 4;
+template <int D>
+constexpr int rows_per_cta() { return 256 / (D / 8) * kRowsPerThread; }
 template <int D>
 __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_constant__ RowsParams p) {
   after_previous();
-  constexpr int kLanes = D / 8;
-  const int64_t r = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  const int lane = threadIdx.x & (kLanes - 1);
-  if (r >= p.rows) return;
-  const int h = static_cast<int>(r % p.heads);
-  const int64_t bl = r / p.heads, b = bl / p.lq_pad;
-  const int l = static_cast<int>(bl - b * p.lq_pad);
-  const int64_t to = (b * p.heads + h) * p.lq_pad + l;
-  float s = 0.f;
-  if (l < p.lq) {
-    float x[8], y[8];
-    unpack8(*reinterpret_cast<const uint4*>(after_previous(p.out) + b * p.so.b + l * p.so.l + h * p.so.h + lane * 8), x);
-    unpack8(*reinterpret_cast<const uint4*>(after_previous(p.dout) + b * p.sdo.b + l * p.sdo.l + h * p.sdo.h + lane * 8), y);
+  constexpr int kLanes = D / 8, kRows = 256 / kLanes;
+  const int lane = threadIdx.x & (kLanes - 1), all = p.lq_pad * p.heads;
+  const int64_t b = blockIdx.y;
+  const int first = blockIdx.x * rows_per_cta<D>() + static_cast<int>(threadIdx.x) / kLanes;
+  const __nv_bfloat16* out = after_previous(p.out) + b * p.so.b + lane * 8;
+  const __nv_bfloat16* dout = after_previous(p.dout) + b * p.sdo.b + lane * 8;
+  uint4 x[kRowsPerThread], y[kRowsPerThread];
+  int l[kRowsPerThread], h[kRowsPerThread];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    const int r = first + i * kRows;
+    l[i] = r / p.heads;
+    h[i] = r - l[i] * p.heads;
+    x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (l[i] < p.lq) {
+      x[i] = ldg_stream16(out + l[i] * p.so.l + h[i] * p.so.h);
+      y[i] = *reinterpret_cast<const uint4*>(dout + l[i] * p.sdo.l + h[i] * p.sdo.h);      // read again by the next two kernels
+    }
   }
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(((1ull << kLanes) - 1) << (threadIdx.x & 31 & ~(kLanes - 1)), s, o);
-  if (lane != 0) return;
-  const float lse = l < p.lq ? after_previous(p.lse)[(b * p.heads + h) * p.lq + l] : -INFINITY;
-  p.lse2[to] = lse == -INFINITY ? -INFINITY : lse * -kLog2e;
-  p.delta[to] = lse == -INFINITY ? 0.f : -s;
+  for (int i = 0; i < kRowsPerThread; ++i) {
+    f2 s = f2_mul(f2_of_bf16(x[i].x), f2_of_bf16(y[i].x));
+    s = f2_fma(f2_of_bf16(x[i].y), f2_of_bf16(y[i].y), s);
+    s = f2_fma(f2_of_bf16(x[i].z), f2_of_bf16(y[i].z), s);
+    s = f2_fma(f2_of_bf16(x[i].w), f2_of_bf16(y[i].w), s);
+    float t = f2_sum(s);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane != 0 || first + i * kRows >= all) continue;
+    const int64_t bh = b * p.heads + h[i], to = bh * p.lq_pad + l[i];
+    const float lse = l[i] < p.lq ? after_previous(p.lse)[bh * p.lq + l[i]] : -INFINITY;
+    p.lse2[to] = lse == -INFINITY ? -INFINITY : lse * -kLog2e;
+    p.delta[to] = lse == -INFINITY ? 0.f : -t;
+  }
 }
 
 // Shared memory: two tiles that stay, a ring (keys: three tiles of q, two of dout with lse2 and delta; queries: five tiles of K
@@ -668,8 +682,9 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
   // as SMs get free ([4, 2047, 16 / 4 heads, 64] 293 -> 270 us; not causal, four rounds cost [8, 4096 x 512] 597 -> 614).
   const int64_t most = (p.z.causal ? 4LL : 1LL) * sm_count();
   auto grid = [&](int64_t items) { return dim3(static_cast<unsigned>(std::min(items, most))); };
-  if (rows.rows) {
-    launch_after(attention_rows_kernel<D>, dim3(static_cast<unsigned>(ceil_div(rows.rows, 256 / (D / 8)))), dim3(256), 0, st, rows);
+  if (plan.row_floats) {
+    const dim3 over(static_cast<unsigned>(ceil_div(plan.lq_pad * s.heads, rows_per_cta<D>())), static_cast<unsigned>(s.batch));
+    launch_after(attention_rows_kernel<D>, over, dim3(256), 0, st, rows);
     ANIMA_CHECK_LAUNCH(who);
   }
   auto join = [&](const float* from, __nv_bfloat16* to, int splits, int64_t elements, int lq) {
@@ -776,7 +791,6 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
   rows.lq = p.z.lq;
   rows.lq_pad = p.lq_pad;
   rows.heads = p.z.heads;
-  rows.rows = s.batch * plan.lq_pad * s.heads;
   const void* stand_in = no_q ? k : q;
   CUtensorMap maps[4];
   ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, stand_in) &&

@@ -112,7 +112,7 @@ inline int check_sizes(const char* who, int64_t batch, int64_t lq, int64_t lk, i
                 (long long)head_dim);
   ANIMA_REQUIRE(heads % kv_heads == 0, ANIMA_E_SHAPE, "%s: heads=%lld is not a multiple of kv_heads=%lld", who,
                 (long long)heads, (long long)kv_heads);
-  ANIMA_REQUIRE(batch < 65536 && heads < 65536 && lq < (1ll << 30) && lk < (1ll << 30) && batch * heads * lq < (1ll << 40),
+  ANIMA_REQUIRE(batch < 65536 && heads < 65536 && lq < (1ll << 30) && lk < (1ll << 30) && heads * lq < (1ll << 30) && batch * heads * lq < (1ll << 40),
                 ANIMA_E_TOO_LARGE, "%s: too large", who);
   return ANIMA_OK;
 }

@@ -179,10 +179,17 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
     float m = -INFINITY, used = 0.f;     // maximum in use (raw scores), m * c (0 while there is none)
     f2 sum[4] = {0ull, 0ull, 0ull, 0ull};
     bool ok = true;
+    // 32 rows behind the last query (a few queries against many keys): nothing is made of their scores, and what lies in their
+    // place in tensor memory only reaches rows of O that nobody stores
+    const bool idle = row - lane >= z.lq;
     for (int u = 0; u < count; ++u) {
       const uint32_t at = s_at + (u & 1) * kStep;
       ok = warp_wait(s_full(u & 1), (u >> 1) & 1, &abort_flag);
       if (!ok) break;
+      if (idle) {
+        if (lane == 0) mbar_arrive(p_full(u & 1));
+        continue;
+      }
       tc_fence_after();
       uint32_t s[2][32];
       tc_ld32(at, s[0]);
