@@ -114,7 +114,8 @@ def run(iters: int, only: str | None, small: bool, pick: str | None = None, dire
     torch.manual_seed(0)
     peaks = _peaks()
     hbm_peak = peaks.get("hbm_gbs")
-    tf_peak = 2.0 * peaks["bf16_tflops"] if "bf16_tflops" in peaks else None  # timed alone: burst figure
+    fp8 = only != "attention"       # attention's products are bf16
+    tf_peak = (2.0 if fp8 else 1.0) * peaks["bf16_tflops"] if "bf16_tflops" in peaks else None  # timed alone: burst figure
     t = Timer(iters, direct=direct)
     out: list[dict] = []
     M = 4096 if small else 32768
@@ -151,9 +152,9 @@ def run(iters: int, only: str | None, small: bool, pick: str | None = None, dire
         ghz = cycles / ns if ns else None
         out.append({"kernel": name, "shape": shape, "ms": round(ms, 4), "bound": "tensor", "achieved": round(tf, 1),
                     "unit": "TFLOP/s", "algorithmic_flops": flops, "peak": tf_peak,
-                    "peak_note": "2 x measured burst bf16 cuBLAS (no measured fp8 figure)",
+                    "peak_note": "2 x measured burst bf16 cuBLAS (no measured fp8 figure)" if fp8 else "measured burst bf16 cuBLAS",
                     "frac_of_measured": round(tf / tf_peak, 3) if tf_peak else None,
-                    "frac_of_nominal_4500": round(tf / 4500.0, 3),
+                    "frac_of_nominal_4500" if fp8 else "frac_of_nominal_2250": round(tf / (4500.0 if fp8 else 2250.0), 3),
                     "sm_mhz_in_kernel": round(ghz * 1000.0) if ghz else None,
                     "tensor_pipe_util_at_that_clock": round(tf * 1e3 / (sms * 16384 * ghz), 3) if ghz else None})
         if cycles:   # share of CTA 0's cycles its warps spent waiting (producer: free stage; issuer: operands,
@@ -234,6 +235,32 @@ def run(iters: int, only: str | None, small: bool, pick: str | None = None, dire
         _, rs = ops.rmsnorm_rope_fwd(q, wn, cos, sin, 1e-6)
         hbm("rmsnorm_rope_fwd", [BT, L, 16, 128], M * D * 4 + M * 16 * 4, lambda: ops.rmsnorm_rope_fwd(q, wn, cos, sin, 1e-6))
         hbm("rmsnorm_rope_bwd", [BT, L, 16, 128], M * D * 6 + M * 16 * 4, lambda: ops.rmsnorm_rope_bwd(dq, q, wn, cos, sin, rs))
+
+    if only == "attention":
+        # Attention of the model's layers (self: 4096 latent tokens; cross: 512 text tokens), causal at half the length, and
+        # what prepares q and k. Backward is counted as five products of two flops a pair and element, as it needs them.
+        H, d = 16, 128
+        bt = M // 4096
+        pairs = {}
+        for name, lq, lk, causal in [("self", 4096, 4096, False), ("cross", 4096, 512, False), ("causal", 2048, 2048, True)]:
+            q, k, v, g = (_acts(bt * n, H * d).view(bt, n, H, d) for n in (lq, lk, lk, lq))
+            o, lse = ops.attention_fwd(q, k, v, causal=causal)
+            pairs[name] = bt * H * (lq * (lq + 1) // 2 if causal else lq * lk)
+            tensor(f"attention fwd {name}", [bt, lq, lk, H, d], 4.0 * d * pairs[name],
+                   lambda: ops.attention_fwd(q, k, v, causal=causal))
+            tensor(f"attention bwd {name}", [bt, lq, lk, H, d], 10.0 * d * pairs[name],
+                   lambda: ops.attention_bwd(g, q, k, v, o, lse, causal=causal))
+            del q, k, v, g, o, lse
+        q1 = _acts(8, H * d).view(8, 1, H, d)
+        kc, vc = (_acts(8 * 8192, 4 * d).view(8, 8192, 4, d) for _ in range(2))
+        hbm("attention fwd, one query on 8192 keys", [8, 1, 8192, H, 4, d], 4 * kc.numel(), lambda: ops.attention_fwd(q1, kc, vc))
+        q, k, gq, gk = (_acts(M, H * d).view(bt, 4096, H, d) for _ in range(4))
+        wn = torch.ones(d, device="cuda")
+        ang = torch.rand(4096, d, device="cuda") * 60
+        cos, sin = ang.cos(), ang.sin()
+        hbm("qk_norm_rope_fwd (q and k)", list(q.shape), 8 * q.numel(), lambda: ops.qk_norm_rope_fwd(q, k, wn, wn, cos, sin, 1e-6))
+        hbm("qk_norm_rope_bwd (with weight gradients)", list(q.shape), 12 * q.numel(),
+            lambda: ops.qk_norm_rope_bwd(gq, gk, q, k, wn, wn, cos, sin, 1e-6))
 
     if only in (None, "tlokr"):
         # The T-LoKr delta of one module, x -> x @ kron(W1, (A * mask) @ B)^T, as the training step runs it: inside
@@ -346,7 +373,7 @@ def summary(iters: int = 8) -> dict:
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--iters", type=int, default=20)
-    ap.add_argument("--only", choices=["gemm", "hbm", "tlokr"], default=None)
+    ap.add_argument("--only", choices=["gemm", "hbm", "tlokr", "attention"], default=None)
     ap.add_argument("--small", action="store_true")
     ap.add_argument("--pick", default=None, help="run only entries whose 'name [shape]' contains this text")
     ap.add_argument("--direct", action="store_true", help="plain launches instead of CUDA-graph replays")

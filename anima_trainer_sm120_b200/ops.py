@@ -8,6 +8,8 @@ from __future__ import annotations
 
 from typing import NamedTuple
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -545,3 +547,100 @@ def rmsnorm_rope_bwd(dout: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
         check(_lib.load().anima_rmsnorm_rope_bwd(ptr(dout), ptr(x), ptr(weight), ptr(cos), ptr(sin), ptr(rstd), tokens,
                                                  heads, d, seq, ptr(dx), _lib.stream_ptr(dev)))
     return dx
+
+
+def _heads(t: torch.Tensor, name: str):
+    """(pointer, strides) of a (batch, tokens, heads, head_dim) bf16 tensor with a dense head vector, read in place."""
+    if t.dtype != BF16 or t.dim() != 4 or (t.shape[3] > 1 and t.stride(3) != 1):
+        raise ValueError(f"{name} must be bfloat16 (batch, tokens, heads, head_dim) with a dense last dimension")
+    return ptr(t), (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def _lengths(n: torch.Tensor | None, batch: int):
+    if n is not None and (n.dtype != torch.int32 or n.shape != (batch,) or not n.is_contiguous()):
+        raise ValueError(f"kv_lengths must be contiguous int32 [{batch}]")
+    return ptr(n)
+
+
+def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lengths: torch.Tensor | None = None,
+                  causal: bool = False, scale: float | None = None, want_lse: bool = True
+                  ) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(out, lse) of q (B, Lq, H, D), k and v (B, Lk, Hk, D): see :func:`attention_kernel.fused_attention`."""
+    dev = _lib.require_cuda(q, k, v, kv_lengths)
+    (B, lq, H, D), (lk, Hk) = q.shape, k.shape[1:3]
+    if k.shape != v.shape or k.shape != (B, lk, Hk, D):
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
+    out = torch.empty((B, lq, H, D), dtype=BF16, device=dev)
+    lse = torch.empty((B, H, lq), dtype=torch.float32, device=dev) if want_lse else None
+    lib, sizes = _lib.load(), (B, lq, lk, H, Hk, D)
+    ws = _lib.workspace(check(lib.anima_attention_fwd_workspace_bytes(*sizes, causal)), dev, "attention_fwd")
+    with torch.cuda.device(dev):
+        check(lib.anima_attention_fwd(*_heads(q, "q"), *_heads(k, "k"), *_heads(v, "v"), _lengths(kv_lengths, B), *sizes,
+                                      float(D ** -0.5 if scale is None else scale), causal, ptr(out), ptr(lse), ptr(ws),
+                                      ws.numel(), ptr(_lib.status_word(dev)), _lib.stream_ptr(dev)))
+    return out, lse
+
+
+def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                  lse: torch.Tensor, *, kv_lengths: torch.Tensor | None = None, causal: bool = False,
+                  scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dq, dk, dv) from what :func:`attention_fwd` took and gave."""
+    dev = _lib.require_cuda(dout, q, k, v, out, lse, kv_lengths)
+    (B, lq, H, D), (lk, Hk) = q.shape, k.shape[1:3]
+    if dout.shape != q.shape or out.shape != q.shape or k.shape != v.shape or k.shape != (B, lk, Hk, D):
+        raise ValueError("attention_bwd: shapes of dout, q, k, v and out do not belong together")
+    if lse.dtype != torch.float32 or lse.shape != (B, H, lq) or not (lse.is_contiguous() and out.is_contiguous()):
+        raise ValueError("attention_bwd needs out and lse as attention_fwd wrote them")
+    dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=dev) for t in (q, k, v))
+    lib, sizes = _lib.load(), (B, lq, lk, H, Hk, D)
+    ws = _lib.workspace(check(lib.anima_attention_bwd_workspace_bytes(*sizes, causal)), dev, "attention_bwd")
+    with torch.cuda.device(dev):
+        check(lib.anima_attention_bwd(*_heads(dout, "dout"), *_heads(q, "q"), *_heads(k, "k"), *_heads(v, "v"), ptr(out), ptr(lse),
+                                      _lengths(kv_lengths, B), *sizes, float(D ** -0.5 if scale is None else scale), causal,
+                                      ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws.numel(), ptr(_lib.status_word(dev)),
+                                      _lib.stream_ptr(dev)))
+    return dq, dk, dv
+
+
+def _qk_args(q, k, q_weight, k_weight, cos, sin, eps):
+    dev = _lib.require_cuda(q, k, q_weight, k_weight, cos, sin)
+    (B, lq, H, D), (lk, Hk) = q.shape, k.shape[1:3]
+    if k.shape != (B, lk, Hk, D) or q_weight.numel() != D or k_weight.numel() != D:
+        raise ValueError(f"k {tuple(k.shape)} and the norm weights do not go with q {tuple(q.shape)}")
+    if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (BF16, torch.float32):
+        raise TypeError("the norm weights must both be bfloat16 or both float32")
+    for t in (cos, sin):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or t.shape[-2:] != (lq, D)):
+            raise ValueError(f"rope tables must be contiguous float32 [..., {lq}, {D}]")
+    samples = cos.shape[0] if cos is not None and cos.dim() == 3 else 1
+    return dev, (*_heads(q, "q"), *_heads(k, "k"), ptr(q_weight.contiguous()), ptr(k_weight.contiguous()),
+                 int(q_weight.dtype == BF16), ptr(cos), ptr(sin), samples, float(eps), B, lq, lk, H, Hk, D)
+
+
+def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                     cos: torch.Tensor | None, sin: torch.Tensor | None, eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """Both results, dense: see :func:`qk_norm_rope.fused_qk_norm_rope`."""
+    dev, args = _qk_args(q, k, q_weight, k_weight, cos, sin, eps)
+    oq, ok = (torch.empty(t.shape, dtype=BF16, device=dev) for t in (q, k))
+    with torch.cuda.device(dev):
+        check(_lib.load().anima_qk_norm_rope_fwd(*args, ptr(oq), ptr(ok), _lib.stream_ptr(dev)))
+    return oq, ok
+
+
+def qk_norm_rope_bwd(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, eps: float, *,
+                     weights: bool = True) -> tuple[torch.Tensor, ...]:
+    """(dq, dk, dq_weight, dk_weight); the weights' gradients are None unless ``weights``."""
+    dev, args = _qk_args(q, k, q_weight, k_weight, cos, sin, eps)
+    if dq_out.shape != q.shape or dk_out.shape != k.shape or not (dq_out.is_contiguous() and dk_out.is_contiguous()):
+        raise ValueError("the incoming gradients must be dense and of q's and k's shapes")
+    _lib.require_cuda(q, dq_out, dk_out)
+    dq, dk = (torch.empty(t.shape, dtype=BF16, device=dev) for t in (q, k))
+    dwq, dwk = (torch.empty_like(w.reshape(-1)) for w in (q_weight, k_weight)) if weights else (None, None)
+    lib, ws = _lib.load(), None
+    if weights:
+        ws = _lib.workspace(check(lib.anima_qk_norm_rope_bwd_workspace_bytes(*args[-6:])), dev, "qk_norm_rope")
+    with torch.cuda.device(dev):
+        check(lib.anima_qk_norm_rope_bwd(ptr(dq_out), ptr(dk_out), *args, ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(ws),
+                                         ws.numel() if weights else 0, _lib.stream_ptr(dev)))
+    return dq, dk, dwq, dwk

@@ -145,3 +145,26 @@ def test_python_entries_refuse_cpu_tensors():
         fused_attention(x, x, x)
     with pytest.raises(RuntimeError, match="CUDA"):
         fused_qk_norm_rope(x, x, x[0, 0, 0], x[0, 0, 0])
+
+
+def test_trainer_options_are_checked_before_anything_is_built():
+    from anima_trainer_sm120_b200.anima_dit import tiny_config
+    from anima_trainer_sm120_b200.train_step import StepConfig, Trainer
+    cpu = torch.device("cpu")
+    with pytest.raises(ValueError, match="attention"):
+        Trainer(tiny_config(), StepConfig(precision="bf16", attention="fused"), cpu)
+    with pytest.raises(ValueError, match="attention"):
+        Trainer(tiny_config(), StepConfig(precision="bf16", attention="other"), cpu)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        Trainer(tiny_config(), StepConfig(precision="bf16_fused", attention="fused"), cpu)
+    Trainer(tiny_config(), StepConfig(precision="bf16", lokr_dim=8, lokr_factor=4), cpu)
+
+
+def test_ops_wrappers_refuse_what_they_cannot_pass_on():
+    from anima_trainer_sm120_b200 import ops
+    x = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16)
+    for call in (lambda: ops.attention_fwd(x, x, x), lambda: ops.attention_bwd(x, x, x, x, x, x),
+                 lambda: ops.qk_norm_rope_fwd(x, x, x[0, 0, 0], x[0, 0, 0], None, None, 1e-6),
+                 lambda: ops.qk_norm_rope_bwd(x, x, x, x, x[0, 0, 0], x[0, 0, 0], None, None, 1e-6)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()

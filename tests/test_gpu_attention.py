@@ -394,3 +394,24 @@ def test_under_checkpoint():
         out.backward(g)
         results.append([out.detach()] + [t.grad for t in leaves])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_thin_wrappers_give_the_nodes_bits():
+    from anima_trainer_sm120_b200 import ops
+    from anima_trainer_sm120_b200.attention_kernel import fused_attention
+    q, k, v, g = _tensors(2, 130, 260, 4, 2, 128, seed=111)
+    n = torch.tensor([260, 99], device=DEV, dtype=torch.int32)
+    out, lse = ops.attention_fwd(q, k, v, kv_lengths=n, causal=True, scale=0.1)
+    grads = ops.attention_bwd(g, q, k, v, out, lse, kv_lengths=n, causal=True, scale=0.1)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want, want_lse = fused_attention(*leaves, kv_lengths=n, causal=True, scale=0.1, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, leaves, g)))
+    with pytest.raises(ValueError):
+        ops.attention_fwd(q, k, v[:, :5])
+    with pytest.raises(ValueError):
+        ops.attention_fwd(q, k, v, kv_lengths=n.long())
+    with pytest.raises(ValueError):
+        ops.attention_bwd(g, q, k, v, out, lse[:1])
+    with pytest.raises(ValueError):
+        ops.attention_fwd(q.transpose(2, 3), k, v)

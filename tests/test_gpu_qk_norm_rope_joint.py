@@ -180,6 +180,25 @@ def test_many_vectors_keep_their_weight_gradient_exact_and_the_same():
     _within("dw", runs[0][2], OA.norm_rope(leaves[0].detach(), leaves[2].detach(), cos, sin, dout=g[0])["dw"])
 
 
+def test_thin_wrappers_give_the_nodes_bits():
+    from anima_trainer_sm120_b200 import ops
+    from anima_trainer_sm120_b200.qk_norm_rope import fused_qk_norm_rope
+    q, k, gq, gk = _rand(1, 2, 30, 6, 64), _rand(2, 2, 30, 2, 64), _rand(3, 2, 30, 6, 64), _rand(4, 2, 30, 2, 64)
+    wq, wk = _rand(5, 64), _rand(6, 64)
+    cos, sin = _tables(7, 2, 30, 64)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, wq, wk)]
+    want = fused_qk_norm_rope(*leaves, cos, sin)
+    grads = torch.autograd.grad(want, leaves, (gq, gk))
+    assert all(torch.equal(a, b) for a, b in zip(ops.qk_norm_rope_fwd(q, k, wq, wk, cos, sin, 1e-6), want))
+    assert all(torch.equal(a, b) for a, b in zip(ops.qk_norm_rope_bwd(gq, gk, q, k, wq, wk, cos, sin, 1e-6), grads))
+    some = ops.qk_norm_rope_bwd(gq, gk, q, k, wq, wk, cos, sin, 1e-6, weights=False)
+    assert torch.equal(some[0], grads[0]) and torch.equal(some[1], grads[1]) and some[2] is None
+    with pytest.raises(TypeError):
+        ops.qk_norm_rope_fwd(q, k, wq, wk.float(), None, None, 1e-6)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope_fwd(q, k, wq, wk, cos[:, :5], sin[:, :5], 1e-6)
+
+
 # ---------------------------------------------------------------------------------------- the layer, the model, the trainer
 @pytest.mark.parametrize("heads", [2, 4])          # head widths 128 and 64
 @pytest.mark.parametrize("cross", [False, True])
