@@ -1,24 +1,28 @@
 // Attention, backward (formulas: attention_common.cuh): the probabilities are made again from q, k and the forward's log-sums.
 //
-// Three launches, no atomics, every sum in a fixed order:
+// No atomics, every sum in a fixed order:
 //   rows   -delta = -out . dout of each query, and minus its log-sum in base 2 (-inf for a query that saw nothing, and for the
 //          rows that fill up the last tile: their probabilities come out as 0);
 //   keys   a CTA takes tiles of 128 keys of a key head and walks, for each, the query tiles of all heads it serves:
-//            S^T = K Q^T, dP^T = V dO^T (lane = key, column = query), dV += P^T dO, dK += dS^T Q;
+//            S^T = K Q^T, dP^T = V dO^T (lane = key, column = query), dV += P^T dO, dK += dS^T Q; dS goes to memory in bf16;
+//   dq     dQ = dS K, a CTA for each tile of 128 queries of a head.
+// Where dS would be too large a kernel makes it again for itself instead of dq:
 //   queries a CTA takes tiles of 128 queries of a head and walks the key tiles for each:
 //            S = Q K^T, dP = dO V^T (lane = query), dQ += dS K.
-// That is 7 products a pair of tiles where one kernel for all three would do 5. It buys this: P^T, dS^T and dS are read by the
-// tensor cores from tensor memory, where the threads that made them wrote them over the scores, and never cross shared memory
-// (whose bandwidth a product with two operands there takes up whole); dQ needs no fp32 buffer that all CTAs add to (atomics
-// whose order would change results, and 4 bytes a key tile and element of traffic), and the sums stay in tensor memory.
+// P^T, dS^T and dS are read by the tensor cores from tensor memory, where the threads that made them wrote them over the scores,
+// and never cross shared memory (whose bandwidth a product with two operands there takes up whole); dQ needs no fp32 buffer that
+// all CTAs add to (atomics whose order would change results, and 4 D bytes a query and key tile, twice those of dS at D = 128).
+// dS costs 4 bytes of traffic a (query, key) pair and saves two products and an exponential (14 -> 10 D flop): [8, 4096, 16, 128]
+// 3.52 -> 3.05 ms, [8, 4096 x 512] 642 -> 530 us, [2, 1024, 16, 128] 83 -> 71 us, [1, 64, 4, 64] 19.5 -> 17.4 us.
 // Each tile of q, dO, K lies in shared memory once and serves as a K-major operand of one product and as an MN-major operand
 // of another.
 // Four warpgroups share a pair of tiles, 32 columns each. One warp issues all products, in the order in which they are waited for
 // (a second one lets dK run between dV and the next S, which all warpgroups wait for: 3000 instead of 2600 cycles a pair): dV(i)
-// and S(i+1) as soon as P(i) lies in tensor memory, dK(i) and dP(i+1) as soon as dS(i) does.
+// and S(i+1) as soon as P(i) lies in tensor memory, dK(i) and dP(i+1) as soon as dS(i) does. A branch around a product that
+// nobody asked for costs the others 10 %: all are made, whichever gradients are wanted.
 // Products of 64 instead of 128 columns would let the halves of a tile take turns, but read their A operand from shared memory
 // twice as often, which then bounds them (1.5 x the time of the same work in whole tiles).
-// Bound: 14 D flop a (query, key) pair on the tensor cores; two exponentials.
+// Bound: keys, shared memory, which the two products with both operands there and the loads of the others keep busy; dq, memory.
 #include "attention_common.cuh"
 
 namespace anima {
@@ -38,6 +42,11 @@ struct BwdParams {
   Strided sdq;                           // dk, dv: dense
   int tiles, splits, per_split;          // key (query) tiles; ranges their walks are cut into, and how long these are
   int items;                             // tiles * splits * heads * batch
+  int first;                             // of the items, where they are a part of all
+  // dS as the tensor cores read it, in tiles [query head - ds_head][query tile][key tile] of kDsTile bytes, null: not stored. A tile:
+  // [half of the keys][8 queries][key][query] bf16.
+  uint8_t* ds;
+  int ds_head, q_tiles, k_tiles;
   float *part0, *part1;                  // fp32 partial sums [split][elements], if splits > 1: dv and dk, or dq
   int64_t elements;
   int32_t* status;
@@ -96,6 +105,11 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
 
 // Shared memory: two tiles that stay, a ring (keys: three tiles of q, two of dout with lse2 and delta; queries: five tiles of K
 // and V), barriers.
+constexpr int kDsTile = kTile * kTile * 2, kDsHalf = kDsTile / 2, kDsGroup = kTile / 2 * 16;     // bytes: a tile, 64 keys of it, 8 queries of these
+__device__ __forceinline__ uint8_t* ds_tile(const BwdParams& p, int head, int qt, int kt) {
+  return p.ds + (static_cast<int64_t>(head - p.ds_head) * p.q_tiles + qt) * p.k_tiles * kDsTile + static_cast<int64_t>(kt) * kDsTile;
+}
+
 template <int D>
 struct BwdCfg {
   static constexpr uint32_t kBytes = tile_bytes<D>();
@@ -282,7 +296,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     // ------------------------------------------------------------ TMA producer: K, V, then q0, dout0 (with lse2, delta), q1, ...
     bool ok = lane == 0;
     bits = ~0u;                            // of the stages' release: all are free at first
-    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       ok = x == 0 || mbar_wait(m.bar(kFixedFree), (x - 1) & 1, &abort_flag);
@@ -309,7 +323,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     bool ok = true;
-    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
@@ -365,7 +379,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint32_t s_at = tmem + lanes + C::kS + wg * 32, dp_at = tmem + lanes + C::kDp + wg * 32;
     const f2 c2 = f2_dup(p.c);
     bool ok = true;
-    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       const int row = w.k0 + (threadIdx.x & 127);
       const bool row_ok = row < w.n;
@@ -421,6 +435,14 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(m.bar(kDsReady));
+        if (p.ds != nullptr) {           // 512 contiguous bytes a warp and store
+          const int key = threadIdx.x & 127;
+          uint8_t* to = ds_tile(p, w.it.b * z.heads + head_at(w, i), tile_at(w, i), w.it.tile) + (key >> 6) * kDsHalf +
+                        wg * 4 * kDsGroup + (key & 63) * 16;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(to + e * kDsGroup) = make_uint4(word[4 * e], word[4 * e + 1], word[4 * e + 2], word[4 * e + 3]);
+        }
       }
       if (ok && w.count > 0) {
         ok = warp_wait(m.bar(kDone), x & 1, &abort_flag);
@@ -431,7 +453,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       __nv_bfloat16* dst = wg < 2 ? p.dv : p.dk;
       float* part = wg < 2 ? p.part0 : p.part1;
       store_row<D / 2>(tmem + lanes + (wg < 2 ? C::kAcc0 : C::kAcc1) + (wg & 1) * (D / 2), w.count > 0, wg < 2 ? 1.f : p.scale,
-                       ok && row < z.lk, dst ? dst + at : nullptr, part ? part + w.it.split * p.elements + at : nullptr);
+                       ok && row < z.lk, dst ? dst + at : nullptr, dst && part ? part + w.it.split * p.elements + at : nullptr);
       if (w.count > 0) {
         tc_fence_before();
         __syncwarp();
@@ -484,7 +506,7 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
     // ------------------------------------------------------------ TMA producer: q, dout, then K0, V0, K1, V1, ...
     bool ok = lane == 0;
     bits = ~0u;                            // of the stages' release: all are free at first
-    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       ok = x == 0 || mbar_wait(m.bar(kFixedFree), (x - 1) & 1, &abort_flag);
@@ -504,7 +526,7 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     bool ok = true;
-    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       auto k_stage = [&](int j) { return 2 * j % C::kStages; };
@@ -550,7 +572,7 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
     const uint32_t dp_at = tmem + lanes + C::kDp + col;
     const f2 c2 = f2_dup(p.c);
     bool ok = true;
-    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
+    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       const int row = w.q0 + (threadIdx.x & 127), h = w.it.head, b = w.it.b;
       const int lim = key_limit(z, w.n, row);
@@ -606,6 +628,133 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
   teardown(&abort_flag, p.status, tmem, warp);
 }
 
+// ------------------------------------------------------------------------------------------------ queries, dS stored: dQ
+// dQ = dS K with the dS that the keys kernel left in memory, which bounds it: [8, 4096, 16, 128] reads 1 GiB in 178 us, 6.0 TB/s.
+// 64 keys a stage; a CTA takes a query tile, or a range of its keys where there are few query tiles; two share an SM, so that one
+// loads while the other stores.
+template <int D>
+struct DqCfg {
+  static constexpr uint32_t kKeyBytes = tile_bytes<D>() / 2, kStageBytes = kDsHalf + kKeyBytes;
+  static constexpr int kStages = D == 128 ? 3 : 4, kBars = 2 * kStages + 1;
+  static constexpr int kSmem = kStages * static_cast<int>(kStageBytes) + kBars * 8 + 24, kThreads = 192;
+  static_assert(2 * (kSmem + 1024) <= 228 * 1024 && kStageBytes >= tile_bytes<D>() / 2, "shared memory of two CTAs");
+};
+template <int D>
+__global__ void __launch_bounds__(DqCfg<D>::kThreads, 2)
+attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_dq,
+                        const __grid_constant__ BwdParams p) {
+  using C = DqCfg<D>;
+  constexpr int kStep = kTile / 2;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem), bars = base + C::kStages * C::kStageBytes, done = bars + 16 * C::kStages;
+  auto stage = [&](int i) { return base + i % C::kStages * C::kStageBytes; };      // K, then dS
+  auto full = [&](int i) { return bars + 8 * (i % C::kStages); };
+  auto empty = [&](int i) { return bars + 8 * (C::kStages + i % C::kStages); };
+  volatile int& abort_flag = *reinterpret_cast<volatile int*>(smem + (bars - base) + C::kBars * 8 + 8);
+  uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(smem + (bars - base) + C::kBars * 8 + 16);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < C::kBars; ++i) mbar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) tc_alloc(smem_u32(&tmem_slot), 128);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  after_previous();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
+
+  const Sizes& z = p.z;
+  const Item it = item_of(p, p.first + p.items - 1 - static_cast<int>(blockIdx.x), z.heads);       // what was stored last may still be in L2
+  const int q0 = it.tile * kTile, n = keys_of(z, it.b), step0 = it.split * p.per_split * 2;      // in steps of 64 keys
+  const int count = min((key_limit(z, n, min(z.lq, q0 + kTile) - 1) + kStep - 1) / kStep - step0, p.per_split * 2);
+  if (warp == 5) {
+    if (lane == 0 && count > 0) {
+      const uint8_t* ds = ds_tile(p, it.b * z.heads + it.head, it.tile, 0) + static_cast<int64_t>(step0) * kDsHalf;
+      for (int i = 0; i < count; ++i) {
+        if (!mbar_wait(empty(i), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
+        mbar_expect_tx(full(i), C::kStageBytes);
+        bulk_load(stage(i) + C::kKeyBytes, ds + static_cast<int64_t>(i) * kDsHalf, kDsHalf, full(i));
+        load_rows<D, kStep>(stage(i), &map_k, full(i), (step0 + i) * kStep, it.head / z.group, it.b);
+      }
+    }
+  } else if (warp == 4) {
+    bool ok = true;
+    for (int i = 0; i < count && ok; ++i) {
+      ok = warp_wait(full(i), (i / C::kStages) & 1, &abort_flag);
+      if (!ok) break;
+      // keys that exist; their rows up to the next multiple of 16 are cleared, the product over the others is left out
+      const int keys = min(kStep, n - (step0 + i) * kStep), steps = (keys + 15) / 16;
+      if (keys & 15) zero_rows<D>(stage(i), kStep * 128, keys, steps * 16);
+      tc_fence_after();
+      const uint64_t k = tc_desc_sw128(stage(i), kStep * 128), ds = tc_desc_plain_mn(stage(i) + C::kKeyBytes, kDsGroup, 128);
+#pragma unroll
+      for (int x = 0; x < kStep / 16; ++x)
+        if (x < steps) tc_mma_ss(tmem, ds + x * (16 * 16 / 16), k + x * (16 * 128 / 16), tc_idesc_bf16(kTile, D, true, true), i > 0 || x > 0);
+      tc_commit_warp(empty(i));
+    }
+    if (ok && count > 0) tc_commit_warp(done);
+  } else {
+    bool ok = true;
+    if (count > 0) {
+      ok = warp_wait(done, 0, &abort_flag);
+      tc_fence_after();
+    }
+    // out through the first stages, which no product reads any more
+    const int r = threadIdx.x, first = q0 + r - lane;
+    const uint32_t to = base + r * 128, from = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    if (p.part0) {
+      const int64_t row = (static_cast<int64_t>(it.b) * z.heads + it.head) * z.lq + q0 + r;
+      store_row<D>(from, count > 0, p.scale, ok && q0 + r < z.lq, nullptr, p.part0 + it.split * p.elements + row * D);
+      ok = false;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      if (p.part0) break;
+      uint32_t o[32];
+      __syncwarp();
+      if (count > 0) {
+        tc_ld32(from + i * 32, o);
+        tc_wait_ld();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[8 * e + x]) * p.scale;
+        const uint4 v = pack8(f);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                     ::"r"(to + (i >> 1) * (kTile * 128) + ((((i & 1) * 4 + e) ^ (r & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                     : "memory");
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0 && ok && first < z.lq) {
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) tma_store_4d(&map_dq, to + c * (kTile * 128), c * 64, first, it.head, it.b);
+      asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+    }
+    __syncwarp();
+  }
+  __syncwarp();
+  if (abort_flag) {
+    // Copies still in flight land before shared memory is released.
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    if (threadIdx.x == 0 && p.status) atomicExch(p.status, 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tc_dealloc(tmem, 128);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ joining the ranges
 // dst[row] = sum over splits of part[split][row] in ascending order; rows of D, one of (batch, head, token) order for dq. Four
 // elements a thread.
@@ -637,34 +786,52 @@ __global__ void __launch_bounds__(256) attention_sum_kernel(const __grid_constan
   *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
 }
 
-// Ranges the work of `ctas` CTAs, `items` passes each, is cut into: two CTAs a SM, none with fewer than four passes; one where
+// Ranges the work of `ctas` CTAs, `items` passes each, is cut into: two CTAs a SM, none with fewer than `least` passes; one where
 // there are CTAs enough.
-int split_count(int64_t ctas, int64_t items) {
+int split_count(int64_t ctas, int64_t items, int64_t least) {
   if (ctas == 0 || ctas >= sm_count()) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(2LL * sm_count(), ctas), items / 4)));
+  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(2LL * sm_count(), ctas), items / least)));
 }
+constexpr int64_t kDsBytes = 1ll << 30;
 struct Plan {
   int64_t lq_pad, row_floats;            // lse2 and delta
   int key_splits, key_per, query_splits, query_per;
   int64_t key_elements, query_elements, key_items, query_items;
-  Plan(const Shape& s, bool want_keys, bool want_queries) {
+  int64_t units, unit_bytes, at_once;    // key heads of all samples; dS of one; those whose dS is stored at a time, 0: it is not
+  explicit Plan(const Shape& s) {
     const int64_t q_tiles = ceil_div(s.lq, kTile), k_tiles = ceil_div(s.lk, kTile), group = s.heads / s.kv_heads;
     lq_pad = q_tiles * kTile;
     row_floats = 2 * s.batch * s.heads * lq_pad;
-    key_splits = want_keys ? split_count(k_tiles * s.kv_heads * s.batch, group * q_tiles) : 1;
+    key_splits = split_count(k_tiles * s.kv_heads * s.batch, group * q_tiles, 4);
     key_per = static_cast<int>(std::max<int64_t>(1, ceil_div(group * q_tiles, key_splits)));
-    query_splits = want_queries ? split_count(q_tiles * s.heads * s.batch, k_tiles) : 1;
-    query_per = static_cast<int>(std::max<int64_t>(1, ceil_div(k_tiles, query_splits)));
     key_elements = s.batch * s.lk * s.kv_heads * s.d;
     query_elements = s.batch * s.lq * s.heads * s.d;
     key_items = k_tiles * key_splits * s.kv_heads * s.batch;
+    // Above kDsBytes dS is stored and read in parts of the key heads, up to four times as large where fewer parts leave fewer
+    // rounds of CTAs half empty ([1, 16384, 16, 128], 2 parts of 8 heads: 6.9 -> 5.6 ms); where the rounds that all parts
+    // together take exceed the undivided ones' by a tenth, making dS again is as fast ([1, 32768, 16, 128], 25.5 ms both) or
+    // faster (causal, tiles of unequal length, [1, 16384, 16 / 4, 64]: 3.0 instead of 3.8 ms in 2 parts, hence a round more).
+    units = s.batch * s.kv_heads;
+    unit_bytes = group * q_tiles * k_tiles * kDsTile;
+    at_once = unit_bytes && unit_bytes <= 4 * kDsBytes ? units : 0;
+    if (at_once * unit_bytes > kDsBytes) {
+      auto rounds = [&](int64_t heads) { return ceil_div(heads * k_tiles * key_splits, sm_count()) + (s.causal ? 1 : 0); };
+      const int64_t least = ceil_div(units, 4 * kDsBytes / unit_bytes);
+      int64_t best = rounds(units) + rounds(units) / 10;
+      at_once = 0;
+      for (int64_t parts = least; parts <= std::min(units, 4 * least); ++parts) {
+        const int64_t each = ceil_div(units, parts), full = units / each, cost = full * rounds(each) + rounds(units - full * each);
+        if (cost <= best) best = cost, at_once = each;
+      }
+    }
+    query_splits = at_once ? split_count(at_once * group * q_tiles, k_tiles, 8) : split_count(q_tiles * s.heads * s.batch, k_tiles, 4);
+    query_per = static_cast<int>(std::max<int64_t>(1, ceil_div(k_tiles, query_splits)));
     query_items = q_tiles * query_splits * s.heads * s.batch;
   }
-  // the partial sums of the keys are read before those of the queries are written: one buffer
-  int64_t part_floats() const {
-    return std::max(key_splits > 1 ? 2 * key_splits * key_elements : 0, query_splits > 1 ? query_splits * query_elements : 0);
-  }
-  int64_t bytes() const { return (row_floats + part_floats()) * 4; }
+  int64_t key_part() const { return key_splits > 1 ? key_splits * key_elements : 0; }
+  int64_t query_part() const { return query_splits > 1 ? query_splits * query_elements : 0; }
+  int64_t floats() const { return (row_floats + 2 * key_part() + query_part() + 63) / 64 * 64; }
+  int64_t bytes() const { return floats() * 4 + at_once * unit_bytes; }
 };
 
 template <int D>
@@ -673,11 +840,12 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
   static PerDeviceOnce once;
   const cudaError_t rc = per_device_once(once, [] {
     cudaError_t e = cudaFuncSetAttribute(attention_bwd_keys_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_bwd_dq_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, DqCfg<D>::kSmem);
     return e ? e : cudaFuncSetAttribute(attention_bwd_queries_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   });
   ANIMA_REQUIRE(rc == cudaSuccess, ANIMA_E_CUDA, "%s: cannot reserve %d bytes of shared memory: %s", who, C::kSmem,
                 cudaGetErrorString(rc));
-  float* part = p.part0;
+  float *ws = const_cast<float*>(p.lse2), *part = p.part0;
   // One CTA a SM goes through all its items; causal, whose items differ in length, four rounds of CTAs, which the GPU hands out
   // as SMs get free ([4, 2047, 16 / 4 heads, 64] 293 -> 270 us; not causal, four rounds cost [8, 4096 x 512] 597 -> 614).
   const int64_t most = (p.z.causal ? 4LL : 1LL) * sm_count();
@@ -693,34 +861,50 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
     ANIMA_CHECK_LAUNCH(who);
     return ANIMA_OK;
   };
-  if ((p.dk || p.dv) && plan.key_elements) {
-    p.splits = plan.key_splits;
-    p.per_split = plan.key_per;
-    p.elements = plan.key_elements;
-    p.part0 = p.splits > 1 ? part : nullptr;
-    p.part1 = p.splits > 1 ? part + p.splits * p.elements : nullptr;
-    p.tiles = static_cast<int>(ceil_div(s.lk, kTile));
-    p.items = static_cast<int>(plan.key_items);
-    launch_after(attention_bwd_keys_kernel<D>, grid(p.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
+  p.q_tiles = static_cast<int>(ceil_div(s.lq, kTile));
+  p.k_tiles = static_cast<int>(ceil_div(s.lk, kTile));
+  BwdParams keys = p, queries = p;
+    keys.tiles = p.k_tiles;
+  keys.splits = plan.key_splits;
+  keys.per_split = plan.key_per;
+  keys.elements = plan.key_elements;
+  keys.part0 = plan.key_part() ? part : nullptr;
+  keys.part1 = plan.key_part() ? part + plan.key_part() : nullptr;
+  queries.tiles = p.q_tiles;
+  queries.splits = plan.query_splits;
+  queries.per_split = plan.query_per;
+  queries.elements = plan.query_elements;
+  queries.part0 = plan.query_part() ? part + 2 * plan.key_part() : nullptr;
+  const bool want_queries = p.dq && plan.query_elements, store = want_queries && plan.at_once;
+  const bool want_keys = ((p.dk || p.dv) && plan.key_elements) || store;
+  if (store) keys.ds = queries.ds = reinterpret_cast<uint8_t*>(ws + plan.floats());
+  const int64_t step = store ? plan.at_once : plan.units, group = s.heads / s.kv_heads;
+  for (int64_t u = 0; want_keys && u < plan.units; u += step) {
+    const int64_t now = std::min(step, plan.units - u);
+    keys.first = static_cast<int>(u * keys.tiles * keys.splits);
+    keys.items = static_cast<int>(now * keys.tiles * keys.splits);
+    keys.ds_head = queries.ds_head = static_cast<int>(u * group);
+    launch_after(attention_bwd_keys_kernel<D>, grid(keys.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], keys);
     ANIMA_CHECK_LAUNCH(who);
-    if (p.splits > 1) {
-      if (p.dv)
-        if (int e = join(p.part0, p.dv, p.splits, p.elements, 0)) return e;
-      if (p.dk)
-        if (int e = join(p.part1, p.dk, p.splits, p.elements, 0)) return e;
-    }
-  }
-  if (p.dq && plan.query_elements) {
-    p.splits = plan.query_splits;
-    p.per_split = plan.query_per;
-    p.elements = plan.query_elements;
-    p.part0 = p.splits > 1 ? part : nullptr;
-    p.tiles = static_cast<int>(ceil_div(s.lq, kTile));
-    p.items = static_cast<int>(plan.query_items);
-    launch_after(attention_bwd_queries_kernel<D>, grid(p.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], p);
+    if (!store) continue;
+    queries.first = static_cast<int>(u * group * queries.tiles * queries.splits);
+    queries.items = static_cast<int>(now * group * queries.tiles * queries.splits);
+    launch_after(attention_bwd_dq_kernel<D>, dim3(static_cast<unsigned>(queries.items)), dim3(DqCfg<D>::kThreads), DqCfg<D>::kSmem, st,
+                 maps[4], maps[5], queries);
     ANIMA_CHECK_LAUNCH(who);
-    if (p.splits > 1) return join(p.part0, p.dq, p.splits, p.elements, p.z.lq);
   }
+  if (want_queries && !plan.at_once) {
+    queries.items = static_cast<int>(plan.query_items);
+    launch_after(attention_bwd_queries_kernel<D>, grid(queries.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], queries);
+    ANIMA_CHECK_LAUNCH(who);
+  }
+  if (keys.part0 && want_keys) {
+    if (p.dv)
+      if (int e = join(keys.part0, p.dv, keys.splits, keys.elements, 0)) return e;
+    if (p.dk)
+      if (int e = join(keys.part1, p.dk, keys.splits, keys.elements, 0)) return e;
+  }
+  if (queries.part0 && want_queries) return join(queries.part0, p.dq, queries.splits, queries.elements, p.z.lq);
   return ANIMA_OK;
 }
 
@@ -733,7 +917,8 @@ using namespace anima;
 extern "C" int64_t anima_attention_bwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
                                                        int64_t head_dim, int causal) {
   if (int rc = attn::check_sizes("attention_bwd", batch, lq, lk, heads, kv_heads, head_dim)) return rc;
-  const attn::Plan plan(attn::Shape(batch, lq, lk, heads, kv_heads, head_dim, causal), true, true);
+  const attn::Shape s(batch, lq, lk, heads, kv_heads, head_dim, causal);
+  const attn::Plan plan(s);
   ANIMA_REQUIRE(plan.key_items < (1ll << 30) && plan.query_items < (1ll << 30), ANIMA_E_TOO_LARGE, "attention_bwd: too many tiles");
   return plan.bytes();
 }
@@ -760,7 +945,7 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
                 who, (long long)workspace_bytes, (long long)need);
   if (no_q && no_k) return ANIMA_OK;
   const attn::Shape s(batch, lq, lk, heads, kv_heads, head_dim, causal);
-  const attn::Plan plan(s, dk || dv, dq != nullptr);
+  const attn::Plan plan(s);
   attn::Strided sq = attn::strided(q_strides), sdo = attn::strided(dout_strides);
   attn::Strided dense = {lq * heads * head_dim, heads * head_dim, head_dim};
   s.regroup(sq);
@@ -792,10 +977,12 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
   rows.lq_pad = p.lq_pad;
   rows.heads = p.z.heads;
   const void* stand_in = no_q ? k : q;
-  CUtensorMap maps[4];
+  CUtensorMap maps[6];                   // q, dout, k, v in whole tiles; K by 64 keys, dq by 32 queries
   ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, stand_in) &&
                     attn::encode_heads(&maps[1], dout, sdo, s.batch, s.lq, s.heads, s.d, stand_in) &&
                     attn::encode_heads(&maps[2], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in) &&
+                    attn::encode_heads(&maps[4], k, attn::strided(k_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in, 64) &&
+                    attn::encode_heads(&maps[5], dq ? dq : stand_in, dense, s.batch, s.lq, s.heads, s.d, stand_in, 32) &&
                     attn::encode_heads(&maps[3], v, attn::strided(v_strides), s.batch, s.lk, s.kv_heads, s.d, stand_in),
                 ANIMA_E_CUDA, "%s: cuTensorMapEncodeTiled failed (driver entry point missing or bad operand)", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -57,12 +57,6 @@ struct FwdParams {
   int32_t* status;
 };
 
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
-               ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-               : "memory");
-}
-
 // grid (q_blocks * splits, heads, batch)
 template <int D>
 __global__ void __launch_bounds__(FwdCfg<D>::kThreads, 2)

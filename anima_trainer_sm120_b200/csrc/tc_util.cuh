@@ -79,9 +79,15 @@ __device__ __forceinline__ uint64_t tc_desc_sw128(uint32_t saddr, uint32_t mn_st
   return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>((mn_step >> 4) & 0x3fffu) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// Instruction descriptor: bf16 x bf16, fp32 accumulator, M x N; A K-major, B K-major or MN-major.
-__host__ __device__ constexpr uint32_t tc_idesc_bf16(int m, int n, bool b_mn_major = false) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+// The same without swizzle, MN-major: 8 elements along M or N are 16 contiguous bytes, 8 K elements 16 bytes apart, the next 8
+// K elements `k_step`, the next 8 along M or N `mn_step` bytes further.
+__device__ __forceinline__ uint64_t tc_desc_plain_mn(uint32_t saddr, uint32_t mn_step, uint32_t k_step) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>((k_step >> 4) & 0x3fffu) << 16) |
+         (static_cast<uint64_t>((mn_step >> 4) & 0x3fffu) << 32) | (1ull << 46);
+}
+// Instruction descriptor: bf16 x bf16, fp32 accumulator, M x N; A and B K-major or MN-major.
+__host__ __device__ constexpr uint32_t tc_idesc_bf16(int m, int n, bool b_mn_major = false, bool a_mn_major = false) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn_major) << 15) | (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
 

@@ -470,7 +470,8 @@ int anima_qk_norm_rope_bwd(const void* dq_out, const void* dk_out, const void* q
  * out dense [batch, lq, heads, head_dim] bf16; lse fp32 [batch, heads, lq] (natural logarithm of the row's sum), NULL: not
  * written (bwd needs it).
  * bwd: dout as q; out and lse as fwd wrote them; dq like q, dk and dv like k, dense; any of them may be NULL. Deterministic.
- * status: device int32 that a kernel raises if one of its bounded waits gave up, or NULL. */
+ * status: device int32 that a kernel raises if one of its bounded waits gave up, or NULL.
+ * The backward's workspace holds dS of the heads that it goes through at a time: 2 bytes a (query, key) pair, 4 GiB at most. */
 int64_t anima_attention_fwd_workspace_bytes(int64_t batch, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
                                             int64_t head_dim, int causal);
 int anima_attention_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,

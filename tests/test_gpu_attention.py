@@ -383,6 +383,46 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(fused_attention(q, k, v), fused_attention(q, *small))
 
 
+def test_gradients_of_many_heads_are_those_of_fewer_heads():
+    """The backward pass goes through 130 heads of 4096 tokens in uneven parts, through 26 at once."""
+    from anima_trainer_sm120_b200.attention_kernel import fused_attention
+    q, k, v, g = _tensors(1, 4096, 4096, 130, 130, 64, seed=61)
+
+    def go(a, b):
+        leaves = [t[:, :, a:b].detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(fused_attention(*leaves), leaves, g[:, :, a:b])
+
+    whole = go(0, 130)
+    for a in range(0, 130, 26):
+        for x, y in zip(whole, go(a, a + 26)):
+            assert torch.equal(x[:, :, a:a + 26], y)
+    _check(q[:, :1000, 129:], k[:, :, 129:], v[:, :, 129:], g[:, :1000, 129:])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_a_key_head_that_serves_very_many_pairs(causal):
+    """16 x 11603 x 11603 pairs to a key head: dS is not stored. Element by element against the 64-bit definition, head by head."""
+    from anima_trainer_sm120_b200.attention_kernel import fused_attention
+    H, L, D = 16, 11603, 64
+    q, k, v, g = _tensors(2, L, L, H, 1, D, seed=71)
+    n = torch.tensor([L, 6001], device=DEV, dtype=torch.int32)
+    k[1, 6001:], v[1, 6001:] = float("nan"), float("inf")
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(fused_attention(*leaves, kv_lengths=n, causal=causal), leaves, g)
+    for b in range(2):
+        sums = {}
+        for h in range(H):
+            want = OA.attention(q[b:b + 1, :, h:h + 1].detach(), k[b:b + 1].detach(), v[b:b + 1].detach(), lengths=n[b:b + 1],
+                                causal=causal, dout=g[b:b + 1, :, h:h + 1])
+            _within("dq", dq[b:b + 1, :, h:h + 1], want["dq"])
+            for name in ("dk", "dv"):
+                value, bound = want[name]
+                sums[name] = (sums[name][0] + value, sums[name][1] + bound) if name in sums else (value, bound)
+        # the sum over heads is rounded to bf16 once, by no more than the half steps of all heads that the bounds count
+        _within("dk", dk[b:b + 1], sums["dk"])
+        _within("dv", dv[b:b + 1], sums["dv"])
+
+
 def test_under_checkpoint():
     from torch.utils.checkpoint import checkpoint
     from anima_trainer_sm120_b200.attention_kernel import fused_attention
