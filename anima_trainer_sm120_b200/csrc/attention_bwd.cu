@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
 // Shared memory: two tiles that stay, a ring (keys: three tiles of q, two of dout with lse2 and delta; queries: five tiles of K
 // and V), barriers.
 constexpr int kDsTile = kTile * kTile * 2, kDsHalf = kDsTile / 2, kDsGroup = kTile / 2 * 16;     // bytes: a tile, 64 keys of it, 8 queries of these
-__device__ __forceinline__ uint8_t* ds_tile(const BwdParams& p, int head, int qt, int kt) {
-  return p.ds + (static_cast<int64_t>(head - p.ds_head) * p.q_tiles + qt) * p.k_tiles * kDsTile + static_cast<int64_t>(kt) * kDsTile;
+__device__ __forceinline__ uint32_t ds_index(const BwdParams& p, int head, int qt, int kt) {       // of 4 GiB / kDsTile tiles at most
+  return (static_cast<uint32_t>(head - p.ds_head) * p.q_tiles + qt) * p.k_tiles + kt;
 }
 
 template <int D>
@@ -378,16 +378,25 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes + C::kS + wg * 32, dp_at = tmem + lanes + C::kDp + wg * 32;
     const f2 c2 = f2_dup(p.c);
+    const uint32_t ds_step = static_cast<uint32_t>(p.k_tiles) * (kDsTile / 16);        // to the next query tile's
     bool ok = true;
     for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       const int row = w.k0 + (threadIdx.x & 127);
       const bool row_ok = row < w.n;
+      // the pass's query tile and the thread's place in the tiles of dS, which the walk goes through in order
+      int qt = 0;
+      uint32_t ds = 0;                   // in 16 bytes
+      if (w.count > 0) {
+        qt = tile_at(w, 0);
+        ds = ds_index(p, w.it.b * z.heads + head_at(w, 0), qt, w.it.tile) * (kDsTile / 16) +
+             (((threadIdx.x >> 6) & 1) * kDsHalf + wg * 4 * kDsGroup) / 16 + (threadIdx.x & 63);
+      }
       for (int i = 0; i < w.count; ++i, ++r) {
         const uint32_t rows = m.row_data(g_at(i)) + wg * 128;
         // queries of these 32 before `from` do not see this key
         int from = row_ok ? 0 : 32;
-        if (z.causal && row_ok) from = row - off - tile_at(w, i) * kTile - wg * 32;
+        if (z.causal && row_ok) from = row - off - qt * kTile - wg * 32;
         const bool edge = __any_sync(0xffffffffu, from > 0);
         ok = warp_wait(m.full(g_at(i)), phase_of(bits, g_at(i)), &abort_flag);
         if (!ok) break;
@@ -435,14 +444,16 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(m.bar(kDsReady));
-        if (p.ds != nullptr) {           // 512 contiguous bytes a warp and store
-          const int key = threadIdx.x & 127;
-          uint8_t* to = ds_tile(p, w.it.b * z.heads + head_at(w, i), tile_at(w, i), w.it.tile) + (key >> 6) * kDsHalf +
-                        wg * 4 * kDsGroup + (key & 63) * 16;
+        if (p.ds != nullptr) {           // 512 contiguous bytes a warp and store (through shared memory and copies: the same time, D = 64 5 % more)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<uint4*>(to + e * kDsGroup) = make_uint4(word[4 * e], word[4 * e + 1], word[4 * e + 2], word[4 * e + 3]);
+            reinterpret_cast<uint4*>(p.ds)[static_cast<uint64_t>(ds) + e * (kDsGroup / 16)] = make_uint4(word[4 * e], word[4 * e + 1], word[4 * e + 2], word[4 * e + 3]);
         }
+        if (++qt == q_tiles) {
+          qt = w.first;
+          ds += w.first * ds_step;
+        }
+        ds += ds_step;
       }
       if (ok && w.count > 0) {
         ok = warp_wait(m.bar(kDone), x & 1, &abort_flag);
@@ -671,7 +682,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const int count = min((key_limit(z, n, min(z.lq, q0 + kTile) - 1) + kStep - 1) / kStep - step0, p.per_split * 2);
   if (warp == 5) {
     if (lane == 0 && count > 0) {
-      const uint8_t* ds = ds_tile(p, it.b * z.heads + it.head, it.tile, 0) + static_cast<int64_t>(step0) * kDsHalf;
+      const uint8_t* ds = p.ds + static_cast<int64_t>(ds_index(p, it.b * z.heads + it.head, it.tile, 0)) * kDsTile + static_cast<int64_t>(step0) * kDsHalf;
       for (int i = 0; i < count; ++i) {
         if (!mbar_wait(empty(i), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;
         mbar_expect_tx(full(i), C::kStageBytes);
