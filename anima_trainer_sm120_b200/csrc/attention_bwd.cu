@@ -141,15 +141,6 @@ enum { kFixedFull = 0, kDone = 1, kSFull = 2, kDpFull = 4, kAccFree = 5, kPReady
 struct Item {
   int split, tile, head, b;
 };
-// Every item takes the stages of a ring from the first on, so that where a pass finds its operands follows from its number in
-// the item alone, which the compiler keeps in uniform registers (with stages counted through all items the products' descriptors
-// went through ordinary ones: 72 instead of 20 cycles an instruction). What carries over from item to item, the phases of the
-// barriers, is one bit each.
-__device__ __forceinline__ uint32_t phase_of(uint32_t& bits, int s) {      // of the next completion of barrier s
-  const uint32_t now = (bits >> s) & 1u;
-  bits ^= 1u << s;
-  return now;
-}
 __device__ __forceinline__ Item item_of(const BwdParams& p, int id, int heads) {
   Item it;
   it.split = id % p.splits;

@@ -71,6 +71,15 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
+// Every item takes the stages of a ring from the first on, so that where a pass finds its operands follows from its number in
+// the item alone, which the compiler keeps in uniform registers (with stages counted through all items the products' descriptors
+// went through ordinary ones: 72 instead of 20 cycles an instruction). What carries over from item to item, the phases of the
+// barriers, is one bit each.
+__device__ __forceinline__ uint32_t phase_of(uint32_t& bits, int s) {      // of the next completion of barrier s
+  const uint32_t now = (bits >> s) & 1u;
+  bits ^= 1u << s;
+  return now;
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"

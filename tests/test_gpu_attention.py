@@ -383,6 +383,17 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(fused_attention(q, k, v), fused_attention(q, *small))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_more_tiles_than_fit_at_once(D, causal):
+    """Two CTAs a SM take all tiles in turn: long, short and empty ones one after the other."""
+    n = torch.tensor([0, 641, 1, 0, 0, 320, 63, 65, 0], device=DEV, dtype=torch.int32)
+    q, k, v, g = _tensors(9, 641, 641, 16, 8, D, seed=81)
+    for b, m in enumerate(n.tolist()):
+        k[b, m:], v[b, m:] = float("nan"), float("inf")
+    _check(q, k, v, g, lengths=n, causal=causal)
+
+
 def test_gradients_of_many_heads_are_those_of_fewer_heads():
     """The backward pass goes through 130 heads of 4096 tokens in uneven parts, through 26 at once."""
     from anima_trainer_sm120_b200.attention_kernel import fused_attention
