@@ -58,10 +58,12 @@ struct RowsParams {
   const float* lse;
   float *lse2, *delta;
   int lq, lq_pad, heads;
+  Divisor by_heads;
 };
 
-// D / 8 lanes a row; a CTA takes kRowsPerCta (token, head) rows of a sample in the order of memory, all loads first. grid (., batch).
-constexpr int kRowsPerThread = 4;
+// D / 8 lanes a row; a CTA takes rows_per_cta (token, head) rows of a sample in the order of memory, all loads first. grid (., batch).
+// Bound: reading out and dout once, [8, 4096, 16, 128] 46.5 us, 5.8 TB/s (with the log-sums loaded last and a division a row 60).
+constexpr int kRowsPerThread = 2;
 template <int D>
 constexpr int rows_per_cta() { return 256 / (D / 8) * kRowsPerThread; }
 template <int D>
@@ -75,13 +77,17 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
   const __nv_bfloat16* dout = after_previous(p.dout) + b * p.sdo.b + lane * 8;
   uint4 x[kRowsPerThread], y[kRowsPerThread];
   int l[kRowsPerThread], h[kRowsPerThread];
+  float lse[kRowsPerThread];
+  const float* lses = after_previous(p.lse);
 #pragma unroll
   for (int i = 0; i < kRowsPerThread; ++i) {
     const int r = first + i * kRows;
-    l[i] = r / p.heads;
+    l[i] = p.by_heads.of(r);
     h[i] = r - l[i] * p.heads;
     x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
+    lse[i] = -INFINITY;
     if (l[i] < p.lq) {
+      if (lane == 0) lse[i] = lses[(b * p.heads + h[i]) * p.lq + l[i]];
       x[i] = ldg_stream16(out + l[i] * p.so.l + h[i] * p.so.h);
       y[i] = *reinterpret_cast<const uint4*>(dout + l[i] * p.sdo.l + h[i] * p.sdo.h);      // read again by the next two kernels
     }
@@ -97,9 +103,8 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
     for (int o = kLanes / 2; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane != 0 || first + i * kRows >= all) continue;
     const int64_t bh = b * p.heads + h[i], to = bh * p.lq_pad + l[i];
-    const float lse = l[i] < p.lq ? after_previous(p.lse)[bh * p.lq + l[i]] : -INFINITY;
-    p.lse2[to] = lse == -INFINITY ? -INFINITY : lse * -kLog2e;
-    p.delta[to] = lse == -INFINITY ? 0.f : -t;
+    p.lse2[to] = lse[i] == -INFINITY ? -INFINITY : lse[i] * -kLog2e;
+    p.delta[to] = lse[i] == -INFINITY ? 0.f : -t;
   }
 }
 
@@ -978,6 +983,7 @@ extern "C" int anima_attention_bwd(const void* dout, const int64_t* dout_strides
   rows.lq = p.z.lq;
   rows.lq_pad = p.lq_pad;
   rows.heads = p.z.heads;
+  rows.by_heads = attn::Divisor(s.heads);
   const void* stand_in = no_q ? k : q;
   CUtensorMap maps[6];                   // q, dout, k, v in whole tiles; K by 64 keys, dq by 32 queries
   ANIMA_REQUIRE(attn::bind_context() && attn::encode_heads(&maps[0], q, sq, s.batch, s.lq, s.heads, s.d, stand_in) &&

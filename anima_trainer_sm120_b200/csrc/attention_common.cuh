@@ -91,6 +91,18 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t sr
                ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
+// n / d for n < 2^31 with one multiplication, rounded up as by Granlund and Montgomery: the hardware has no division of integers,
+// and the four of an item's place made a short call 0.3 us longer.
+struct Divisor {
+  uint32_t mul = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(int64_t d) {
+    while ((1ll << shift) < d) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int of(int n) const { return static_cast<int>((__umulhi(n, mul) + n) >> shift); }
+};
+
 // ROWS tokens of one head: D / 64 chunks of ROWS x 128 bytes (swizzled), one behind the other. Tokens behind the last one arrive
 // as zeros.
 template <int D, int ROWS>

@@ -49,18 +49,6 @@ struct FwdCfg {
   static constexpr uint32_t kS = 0, kO = kTile, kCols = 256;
 };
 
-// n / d for n < 2^31 with one multiplication, rounded up as by Granlund and Montgomery: the hardware has no division of integers,
-// and the four of an item's place made a short call 0.3 us longer.
-struct Divisor {
-  uint32_t mul = 0, shift = 0;
-  Divisor() = default;
-  explicit Divisor(int64_t d) {
-    while ((1ll << shift) < d) ++shift;
-    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ int of(int n) const { return static_cast<int>((__umulhi(n, mul) + n) >> shift); }
-};
-
 struct FwdParams {
   Sizes z;
   float c;                               // scale * log2 e
