@@ -15,7 +15,7 @@ _PATCHED: dict[type, object] = {}
 
 def _patched_attend(self, q, k, v, attn_params=None):
     if not (q.is_cuda and q.dtype == k.dtype == v.dtype == torch.bfloat16 and q.shape[-1] in (64, 128)):
-        return _PATCHED[type(self)](self, q, k, v, attn_params)
+        return next(_PATCHED[c] for c in type(self).__mro__ if c in _PATCHED)(self, q, k, v, attn_params)
     return fused_attention(q, k, v, kv_lengths=self._key_lengths(attn_params))
 
 

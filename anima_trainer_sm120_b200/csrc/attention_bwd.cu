@@ -821,7 +821,7 @@ struct Plan {
     units = s.batch * s.kv_heads;
     unit_bytes = group * q_tiles * k_tiles * kDsTile;
     at_once = unit_bytes && unit_bytes <= 4 * kDsBytes ? units : 0;
-    if (at_once * unit_bytes > kDsBytes) {
+    if (at_once && units > kDsBytes / unit_bytes) {
       auto rounds = [&](int64_t heads) { return ceil_div(heads * k_tiles * key_splits, sm_count()) + (s.causal ? 1 : 0); };
       const int64_t least = ceil_div(units, 4 * kDsBytes / unit_bytes);
       int64_t best = rounds(units) + rounds(units) / 10;

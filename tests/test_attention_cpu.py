@@ -168,3 +168,21 @@ def test_ops_wrappers_refuse_what_they_cannot_pass_on():
                  lambda: ops.qk_norm_rope_bwd(x, x, x, x, x[0, 0, 0], x[0, 0, 0], None, None, 1e-6)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_patch_reaches_a_class_derived_from_the_patched_one():
+    from anima_trainer_sm120_b200 import attention_patch
+    from anima_trainer_sm120_b200.anima_dit import AnimaConfig, Attention
+
+    class Derived(Attention):
+        pass
+
+    cfg = AnimaConfig(dim=128, heads=2, depth=1)
+    module = Derived(cfg, None)
+    q, k, v = (torch.randn(1, 5, 2, cfg.head_dim) for _ in range(3))
+    want = module._attend(q, k, v)
+    attention_patch.install(Attention)
+    try:
+        assert torch.equal(module._attend(q, k, v), want)          # CPU tensors: the original method
+    finally:
+        attention_patch.uninstall(Attention)
