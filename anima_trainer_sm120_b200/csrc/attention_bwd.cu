@@ -41,8 +41,8 @@ struct BwdParams {
   __nv_bfloat16 *dq, *dk, *dv;
   Strided sdq;                           // dk, dv: dense
   int tiles, splits, per_split;          // key (query) tiles; ranges their walks are cut into, and how long these are
-  int items;                             // tiles * splits * heads * batch
-  int first;                             // of the items, where they are a part of all
+  int head0, heads_now, items;           // the launch's first head of those of all samples, their number; tiles * splits * heads_now
+  int block, last_first;                 // heads that the items go through together; from the last tile on
   // dS as the tensor cores read it, in tiles [query head - ds_head][query tile][key tile] of kDsTile bytes, null: not stored. A tile:
   // [half of the keys][8 queries][key][query] bf16.
   uint8_t* ds;
@@ -141,16 +141,25 @@ enum { kFixedFull = 0, kDone = 1, kSFull = 2, kDpFull = 4, kAccFree = 5, kPReady
 
 // One item of a CTA's work: range `split` of the walk of one tile. The CTAs go through the items in turn, so that the loads and
 // first products of an item overlap the last passes and the way out of the one before. Causal, the tiles' walks differ in
-// length: their order turns by one from head to head, or a CTA would meet the same ones again and again. 32-bit arithmetic: a
-// 64-bit division is a call, behind which the compiler takes nothing for uniform any more (see phase_of; 761 became 873 us).
+// length: the items go through blocks of heads, the longest walks of all its heads first, so that the short ones fill what is
+// left ([4, 2047, 16 / 4, 64] 216 -> 170 us, [1, 16384, 16 / 4, 64] 3.03 -> 2.27 ms, [8, 2048, 16, 128] 498 -> 480 us). Few enough heads that
+// what they read stays in L2. 32-bit arithmetic: a 64-bit division is a call, behind which the
+// compiler takes nothing for uniform any more (see phase_of; 761 became 873 us).
 struct Item {
   int split, tile, head, b;
 };
 __device__ __forceinline__ Item item_of(const BwdParams& p, int id, int heads) {
   Item it;
   it.split = id % p.splits;
-  const int rest = id / p.splits, bh = rest / p.tiles;
-  it.tile = (rest + (p.z.causal ? bh % p.tiles : 0)) % p.tiles;
+  const int rest = id / p.splits;
+  int bh = rest / p.tiles, x = rest - bh * p.tiles;
+  if (p.block > 1) {
+    const int block = bh / p.block, here = min(p.block, p.heads_now - block * p.block), r = rest - block * p.block * p.tiles;
+    x = r / here;
+    bh = block * p.block + r - x * here;
+  }
+  bh += p.head0;
+  it.tile = p.last_first ? p.tiles - 1 - x : x;
   it.head = bh % heads;
   it.b = bh / heads;
   return it;
@@ -292,7 +301,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     // ------------------------------------------------------------ TMA producer: K, V, then q0, dout0 (with lse2, delta), q1, ...
     bool ok = lane == 0;
     bits = ~0u;                            // of the stages' release: all are free at first
-    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       ok = x == 0 || mbar_wait(m.bar(kFixedFree), (x - 1) & 1, &abort_flag);
@@ -319,7 +328,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     bool ok = true;
-    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       // Causal, more queries than keys: the first -off queries see nothing. Whole tiles of them are not walked; in the tile they
@@ -376,7 +385,7 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const f2 c2 = f2_dup(p.c);
     const uint32_t ds_step = static_cast<uint32_t>(p.k_tiles) * (kDsTile / 16);        // to the next query tile's
     bool ok = true;
-    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       const int row = w.k0 + (threadIdx.x & 127);
       const bool row_ok = row < w.n;
@@ -513,7 +522,7 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
     // ------------------------------------------------------------ TMA producer: q, dout, then K0, V0, K1, V1, ...
     bool ok = lane == 0;
     bits = ~0u;                            // of the stages' release: all are free at first
-    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       ok = x == 0 || mbar_wait(m.bar(kFixedFree), (x - 1) & 1, &abort_flag);
@@ -533,7 +542,7 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     bool ok = true;
-    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       if (w.count == 0) continue;
       auto k_stage = [&](int j) { return 2 * j % C::kStages; };
@@ -579,7 +588,7 @@ attention_bwd_queries_kernel(const __grid_constant__ CUtensorMap map_q, const __
     const uint32_t dp_at = tmem + lanes + C::kDp + col;
     const f2 c2 = f2_dup(p.c);
     bool ok = true;
-    for (int id = p.first + blockIdx.x; id < p.first + p.items && ok; id += gridDim.x) {
+    for (int id = blockIdx.x; id < p.items && ok; id += gridDim.x) {
       const Walk w = walk_of(id);
       const int row = w.q0 + (threadIdx.x & 127), h = w.it.head, b = w.it.b;
       const int lim = key_limit(z, w.n, row);
@@ -673,7 +682,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
   const Sizes& z = p.z;
-  const Item it = item_of(p, p.first + p.items - 1 - static_cast<int>(blockIdx.x), z.heads);       // what was stored last may still be in L2
+  const Item it = item_of(p, p.items - 1 - static_cast<int>(blockIdx.x), z.heads);       // what was stored last may still be in L2
   const int q0 = it.tile * kTile, n = keys_of(z, it.b), step0 = it.split * p.per_split * 2;      // in steps of 64 keys
   const int count = min((key_limit(z, n, min(z.lq, q0 + kTile) - 1) + kStep - 1) / kStep - step0, p.per_split * 2);
   if (warp == 5) {
@@ -817,7 +826,7 @@ struct Plan {
     // Above kDsBytes dS is stored and read in parts of the key heads, up to four times as large where fewer parts leave fewer
     // rounds of CTAs half empty ([1, 16384, 16, 128], 2 parts of 8 heads: 6.9 -> 5.6 ms); where the rounds that all parts
     // together take exceed the undivided ones' by a tenth, making dS again is as fast ([1, 32768, 16, 128], 25.5 ms both) or
-    // faster (causal, tiles of unequal length, [1, 16384, 16 / 4, 64]: 3.0 instead of 3.8 ms in 2 parts, hence a round more).
+    // faster (causal, tiles of unequal length, [1, 16384, 16 / 4, 64]: 2.3 instead of 3.5 ms in 2 parts, hence a round more).
     units = s.batch * s.kv_heads;
     unit_bytes = group * q_tiles * k_tiles * kDsTile;
     at_once = unit_bytes && unit_bytes <= 4 * kDsBytes ? units : 0;
@@ -886,22 +895,27 @@ int launch(const char* who, const CUtensorMap* maps, const Plan& plan, const Sha
   const bool want_keys = ((p.dk || p.dv) && plan.key_elements) || store;
   if (store) keys.ds = queries.ds = reinterpret_cast<uint8_t*>(ws + plan.floats());
   const int64_t step = store ? plan.at_once : plan.units, group = s.heads / s.kv_heads;
+  auto heads_of = [&](BwdParams& q, int64_t head0, int64_t heads) {
+    q.head0 = static_cast<int>(head0);
+    q.heads_now = static_cast<int>(heads);
+    q.items = static_cast<int>(heads * q.tiles * q.splits);
+    q.block = p.z.causal ? static_cast<int>(ceil_div(4LL * sm_count(), q.tiles)) : 1;
+  };
   for (int64_t u = 0; want_keys && u < plan.units; u += step) {
     const int64_t now = std::min(step, plan.units - u);
-    keys.first = static_cast<int>(u * keys.tiles * keys.splits);
-    keys.items = static_cast<int>(now * keys.tiles * keys.splits);
+    heads_of(keys, u, now);
     keys.ds_head = queries.ds_head = static_cast<int>(u * group);
     launch_after(attention_bwd_keys_kernel<D>, grid(keys.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], keys);
     ANIMA_CHECK_LAUNCH(who);
     if (!store) continue;
-    queries.first = static_cast<int>(u * group * queries.tiles * queries.splits);
-    queries.items = static_cast<int>(now * group * queries.tiles * queries.splits);
+    heads_of(queries, u * group, now * group);
     launch_after(attention_bwd_dq_kernel<D>, dim3(static_cast<unsigned>(queries.items)), dim3(DqCfg<D>::kThreads), DqCfg<D>::kSmem, st,
                  maps[4], maps[5], queries);
     ANIMA_CHECK_LAUNCH(who);
   }
   if (want_queries && !plan.at_once) {
-    queries.items = static_cast<int>(plan.query_items);
+    heads_of(queries, 0, plan.units * group);
+    queries.last_first = p.z.causal;
     launch_after(attention_bwd_queries_kernel<D>, grid(queries.items), dim3(kThreads), C::kSmem, st, maps[0], maps[1], maps[2], maps[3], queries);
     ANIMA_CHECK_LAUNCH(who);
   }
