@@ -394,20 +394,28 @@ def test_more_tiles_than_fit_at_once(D, causal):
     _check(q, k, v, g, lengths=n, causal=causal)
 
 
-def test_gradients_of_many_heads_are_those_of_fewer_heads():
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_many_heads_are_those_of_fewer_heads(causal):
     """The backward pass goes through 130 heads of 4096 tokens in uneven parts, through 26 at once."""
     from anima_trainer_sm120_b200.attention_kernel import fused_attention
     q, k, v, g = _tensors(1, 4096, 4096, 130, 130, 64, seed=61)
 
     def go(a, b):
         leaves = [t[:, :, a:b].detach().requires_grad_(True) for t in (q, k, v)]
-        return torch.autograd.grad(fused_attention(*leaves), leaves, g[:, :, a:b])
+        return torch.autograd.grad(fused_attention(*leaves, causal=causal), leaves, g[:, :, a:b])
 
     whole = go(0, 130)
     for a in range(0, 130, 26):
         for x, y in zip(whole, go(a, a + 26)):
             assert torch.equal(x[:, :, a:a + 26], y)
-    _check(q[:, :1000, 129:], k[:, :, 129:], v[:, :, 129:], g[:, :1000, 129:])
+    _check(q[:, :1000, 129:], k[:, :, 129:], v[:, :, 129:], g[:, :1000, 129:], causal=causal)
+
+
+def test_causal_heads_in_several_blocks():
+    """The tiles of several hundred heads are taken in turn; 656 heads are more than one such block, and not a whole number."""
+    n = torch.tensor([130 - i for i in range(41)], device=DEV, dtype=torch.int32)
+    _check(*_tensors(41, 130, 130, 16, 16, 64, seed=91), lengths=n, causal=True)
+    _check(*_tensors(41, 130, 259, 16, 8, 64, seed=92), causal=True)
 
 
 @pytest.mark.parametrize("causal", [False, True])
