@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(256) attention_rows_kernel(const __grid_consta
 
 // Shared memory: two tiles that stay, a ring (keys: three tiles of q, two of dout with lse2 and delta; queries: five tiles of K
 // and V), barriers.
-constexpr int kDsTile = kTile * kTile * 2, kDsHalf = kDsTile / 2, kDsGroup = kTile / 2 * 16;     // bytes: a tile, 64 keys of it, 8 queries of these
+// bytes: a tile, 64 keys of it, 8 queries of these
+constexpr int kDsTile = kTile * kTile * 2, kDsHalf = kDsTile / 2, kDsGroup = kTile / 2 * 16;
 __device__ __forceinline__ uint32_t ds_index(const BwdParams& p, int head, int qt, int kt) {       // of 4 GiB / kDsTile tiles at most
   return (static_cast<uint32_t>(head - p.ds_head) * p.q_tiles + qt) * p.k_tiles + kt;
 }
@@ -449,7 +450,8 @@ attention_bwd_keys_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(m.bar(kDsReady));
-        if (p.ds != nullptr) {           // 512 contiguous bytes a warp and store (through shared memory and copies: the same time, D = 64 5 % more)
+        // 512 contiguous bytes a warp and store (through shared memory and copies: the same time, D = 64 5 % more)
+        if (p.ds != nullptr) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             reinterpret_cast<uint4*>(p.ds)[static_cast<uint64_t>(ds) + e * (kDsGroup / 16)] = make_uint4(word[4 * e], word[4 * e + 1], word[4 * e + 2], word[4 * e + 3]);
@@ -687,6 +689,7 @@ attention_bwd_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
   const int count = min((key_limit(z, n, min(z.lq, q0 + kTile) - 1) + kStep - 1) / kStep - step0, p.per_split * 2);
   if (warp == 5) {
     if (lane == 0 && count > 0) {
+      asm volatile("fence.proxy.async.global;" ::: "memory");      // dS was written by ordinary stores
       const uint8_t* ds = p.ds + static_cast<int64_t>(ds_index(p, it.b * z.heads + it.head, it.tile, 0)) * kDsTile + static_cast<int64_t>(step0) * kDsHalf;
       for (int i = 0; i < count; ++i) {
         if (!mbar_wait(empty(i), ((i / C::kStages) & 1) ^ 1, &abort_flag)) break;

@@ -318,8 +318,8 @@ attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_con
         }
       } else {
         if (live && p.lse) p.lse[at] = total * kLn2;
-        // by way of shared memory, 64 columns at a time, swizzled as TMA wants it; rows behind the last query are left out by the store
-                const int first = row - lane;              // of the warp's 32 rows
+        // by way of shared memory, swizzled as TMA wants it; rows behind the last query are left out by the store
+        const int first = row - lane;            // of the warp's 32 rows
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
           uint32_t o[2][32];
