@@ -435,11 +435,12 @@ int launch_fwd(const char* who, const CUtensorMap* maps, const FwdParams& p, cud
 }
 template <int D>
 int launch(const char* who, const CUtensorMap* maps, const FwdParams& p, const Shape& s, cudaStream_t st) {
-  // Up to 16 steps a tile, two CTAs a SM take all tiles in turn. Above, what that saves is less than what sharing the tiles out
-  // beforehand costs, when a SM has two CTAs with one more than the others ([2, 4096 x 4096] run after run 295 instead of 276 us;
-  // causal, tiles of unequal length, [4, 2047, 16 / 4, 64] 83 / 75): each has its own CTA, taken by the SM that is free first.
-  const int64_t steps = ceil_div(ceil_div(s.lk, kStep), p.splits);
-  const bool stay = !p.z.causal && steps <= 16 && p.items > 2LL * sm_count();
+  // Where a tile has up to 32 steps, or there are six tiles a CTA, two CTAs a SM take all tiles in turn ([4, 4096 x 1536] 224 -> 204 us,
+  // [4, 4096 x 4096, 16, 64] 407 -> 391). Else what that saves is less than what sharing the tiles out beforehand costs, when a SM
+  // has two CTAs with one more than the others ([2, 4096 x 4096] run after run 290 instead of 267 us; causal, tiles of unequal
+  // length, [4, 2047, 16 / 4, 64] 83 / 75): each has its own CTA, taken by the SM that is free first.
+  const int64_t steps = ceil_div(ceil_div(s.lk, kStep), p.splits), slots = 2LL * sm_count();
+  const bool stay = !p.z.causal && p.items > slots && (steps <= 32 || p.items >= 6 * slots);
   if (int e = stay ? launch_fwd<D, true>(who, maps, p, st) : launch_fwd<D, false>(who, maps, p, st)) return e;
   if (p.splits > 1) {
     launch_after(attention_join_kernel<D>, dim3(static_cast<unsigned>(ceil_div(p.rows, 8))), dim3(256), 0, st, p);
